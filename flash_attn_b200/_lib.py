@@ -12,11 +12,14 @@ LIB_PATH = os.path.join(PKG, "libfa_b200.so")
 FA_DTYPE_FP16, FA_DTYPE_BF16, FA_DTYPE_FP32 = 0, 1, 2
 FA_OK = 0
 FA_ACCUM_FIRST, FA_ACCUM_FINAL = 1, 2
+FA_ROTARY_PLAIN, FA_ROTARY_LINEAR, FA_ROTARY_NTK, FA_ROTARY_RAMP = 0, 1, 2, 3
+FA_STATUS_PAGE = 400
 
 #: every symbol include/fa_b200.h declares
 EXPORTS = ["fa_fwd", "fa_fwd_workspace_bytes", "fa_fwd_resolve_splits", "fa_fwd_plan", "fa_num_splits_heuristic",
            "fa_dropout_mask", "fa_merge_partial", "fa_cast_output", "fa_fwd_host", "fa_fwd_host_release",
            "fa_fwd_static_scratch", "fa_static_scratch_bytes", "fa_launch_reference_params", "fa_strerror", "fa_version",
+           "fa_rotary_frequencies", "fa_rotary", "fa_paged_append", "fa_paged_fwd", "fa_paged_fwd_workspace_bytes",
            "fa_ring_fwd", "fa_ring_message_bytes", "fa_ring_unique_id", "fa_ring_comm_create", "fa_ring_comm_destroy"]
 
 
@@ -68,6 +71,61 @@ class RingParams(ctypes.Structure):
         ("accum_o", ctypes.c_void_p * 2), ("accum_lse", ctypes.c_void_p * 2),
         ("compute_stream", ctypes.c_void_p), ("comm_stream", ctypes.c_void_p),
         ("status", ctypes.c_void_p),
+    ]
+
+
+class PagedKv(ctypes.Structure):
+    """struct fa_paged_kv"""
+    _fields_ = [
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+        ("dtype", ctypes.c_int), ("num_pages", ctypes.c_int), ("page_size", ctypes.c_int),
+        ("heads", ctypes.c_int), ("head_dim", ctypes.c_int),
+        ("k_stride", ctypes.c_int64 * 3), ("v_stride", ctypes.c_int64 * 3),
+        ("page_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+        ("table_width", ctypes.c_int), ("batch", ctypes.c_int),
+        ("seqlens_k", ctypes.c_void_p), ("cu_seqlens_q", ctypes.c_void_p),
+    ]
+
+
+class RotaryParams(ctypes.Structure):
+    """struct fa_rotary_params"""
+    _fields_ = [
+        ("x", ctypes.c_void_p), ("y", ctypes.c_void_p),
+        ("dtype", ctypes.c_int), ("batch", ctypes.c_int), ("heads", ctypes.c_int), ("rows", ctypes.c_int),
+        ("head_dim", ctypes.c_int), ("rotary_dim", ctypes.c_int),
+        ("x_stride", ctypes.c_int64 * 3), ("y_stride", ctypes.c_int64 * 3),
+        ("positions", ctypes.c_void_p), ("positions_64", ctypes.c_int), ("position_stride", ctypes.c_int64),
+        ("inv_freq", ctypes.c_void_p), ("amplitude", ctypes.c_float),
+        ("interleaved", ctypes.c_int), ("inverse", ctypes.c_int),
+        ("stream", ctypes.c_void_p),
+    ]
+
+
+class PagedAppendParams(ctypes.Structure):
+    """struct fa_paged_append_params"""
+    _fields_ = [
+        ("cache", PagedKv),
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("q", ctypes.c_void_p), ("q_out", ctypes.c_void_p),
+        ("tokens", ctypes.c_int64), ("heads", ctypes.c_int),
+        ("k_new_stride", ctypes.c_int64 * 2), ("v_new_stride", ctypes.c_int64 * 2),
+        ("q_stride", ctypes.c_int64 * 2), ("q_out_stride", ctypes.c_int64 * 2),
+        ("rotary_dim", ctypes.c_int), ("inv_freq", ctypes.c_void_p), ("amplitude", ctypes.c_float), ("interleaved", ctypes.c_int),
+        ("status", ctypes.c_void_p), ("stream", ctypes.c_void_p),
+    ]
+
+
+class PagedFwdParams(ctypes.Structure):
+    """struct fa_paged_fwd_params"""
+    _fields_ = [
+        ("cache", PagedKv),
+        ("q", ctypes.c_void_p), ("o", ctypes.c_void_p), ("lse", ctypes.c_void_p),
+        ("o_dtype", ctypes.c_int), ("heads", ctypes.c_int), ("tokens", ctypes.c_int64),
+        ("q_stride", ctypes.c_int64 * 2), ("o_stride", ctypes.c_int64 * 2),
+        ("max_seqlen_q", ctypes.c_int), ("softmax_scale", ctypes.c_float),
+        ("is_causal", ctypes.c_int), ("window_left", ctypes.c_int), ("window_right", ctypes.c_int),
+        ("alibi_slopes", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+        ("status", ctypes.c_void_p), ("stream", ctypes.c_void_p),
     ]
 
 
@@ -130,6 +188,17 @@ def load():
     L.fa_merge_partial.restype = ctypes.c_int
     L.fa_cast_output.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_void_p]
     L.fa_cast_output.restype = ctypes.c_int
+    L.fa_rotary_frequencies.argtypes = [ctypes.c_int, ctypes.c_double, ctypes.c_int] + [ctypes.c_double] * 4 + [
+        ctypes.POINTER(ctypes.c_double)] * 2
+    L.fa_rotary_frequencies.restype = ctypes.c_int
+    L.fa_rotary.argtypes = [ctypes.POINTER(RotaryParams)]
+    L.fa_rotary.restype = ctypes.c_int
+    L.fa_paged_append.argtypes = [ctypes.POINTER(PagedAppendParams)]
+    L.fa_paged_append.restype = ctypes.c_int
+    L.fa_paged_fwd.argtypes = [ctypes.POINTER(PagedFwdParams)]
+    L.fa_paged_fwd.restype = ctypes.c_int
+    L.fa_paged_fwd_workspace_bytes.argtypes = [ctypes.POINTER(PagedFwdParams)]
+    L.fa_paged_fwd_workspace_bytes.restype = ctypes.c_size_t
     rp = ctypes.POINTER(RingParams)
     L.fa_ring_fwd.argtypes = [rp]
     L.fa_ring_fwd.restype = ctypes.c_int
@@ -150,13 +219,13 @@ def load():
     return L
 
 
-forward = None  # the call path on torch tensors, once load_call has run
+forward = rotary = append = paged = None  # the call paths on torch tensors, once load_call has run
 
 
 def load_call():
-    """The call path on torch tensors (csrc/fa_torch.cpp), bound to the library's entry points.  Only flash_attn_forward needs
-    it: a module that is missing or was built for another torch leaves the C entry points usable."""
-    global forward
+    """The call paths on torch tensors (csrc/fa_torch.cpp), bound to the library's entry points.  Only flash_attn_forward and the
+    calls around a paged cache need them: a module that is missing or was built for another torch leaves the C entry points usable."""
+    global forward, rotary, append, paged
     L = load()
     import torch
     built = "build it with `python -m flash_attn_b200.build`"
@@ -166,7 +235,11 @@ def load_call():
         raise ImportError(f"the call path on torch tensors cannot be loaded ({e}): {built}") from e
     if _call.built_for != torch.__version__:
         raise ImportError(f"the call path was built for torch {_call.built_for}, this is {torch.__version__}: {built}")
-    forward = functools.partial(_call.forward, *(ctypes.cast(f, ctypes.c_void_p).value for f in (L.fa_fwd, L.fa_fwd_workspace_bytes)))
+    bound = lambda call, *entries: functools.partial(call, *(ctypes.cast(f, ctypes.c_void_p).value for f in entries))  # noqa: E731
+    rotary = bound(_call.rotary, L.fa_rotary)
+    append = bound(_call.append, L.fa_paged_append)
+    paged = bound(_call.paged, L.fa_paged_fwd, L.fa_paged_fwd_workspace_bytes)
+    forward = bound(_call.forward, L.fa_fwd, L.fa_fwd_workspace_bytes)
     return forward
 
 

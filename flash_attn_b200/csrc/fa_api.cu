@@ -12,6 +12,7 @@
 #include <cuda_runtime.h>
 #include "../../include/fa_b200.h"
 #include "fa_internal.h"
+#include "fa_paged.h"
 
 namespace {
 
@@ -354,6 +355,8 @@ int run_fwd(const fa_fwd_params* p, int o_dim, int splits, int sms) {
 }
 
 }  // namespace
+
+int fa::current_device(int* sms, int* major) { return sm_count_of_current_device(sms, major); }
 
 extern "C" {
 

@@ -299,6 +299,126 @@ int fa_ring_unique_id(void* id_out, size_t bytes);
 int fa_ring_comm_create(void** comm_out, int world, int rank, const void* id, size_t bytes);
 int fa_ring_comm_destroy(void* comm);
 
+/*
+ * A paged K/V cache, and the three calls of a layer that serves from it: rotary positions, the append of new
+ * tokens, and their attention over what the cache holds.  No counterpart in the reference, which has K and V in
+ * one piece (src/main.cu:82-107).
+ *
+ * The cache is a pool of num_pages pages, each room for page_size tokens of every K/V head.  Sequence b has
+ * seqlens_k[b] tokens in it, the new ones of this step included; token t lies in page page_table[b][t / page_size],
+ * slot t % page_size.  The new tokens of all sequences are rows one behind the other: those of sequence b are rows
+ * cu_seqlens_q[b] .. cu_seqlens_q[b + 1] - 1 (with cu_seqlens_q NULL: row b alone), and take the last positions of the
+ * sequence: the j-th of n has position seqlens_k[b] - n + j.  Rows outside of every sequence (a padded batch) are left
+ * as they were.  Lengths and tables are read on the device when the call's turn in the stream comes, so that a captured
+ * call is replayed on new ones.
+ * Whatever they hold, no memory outside the tensors is touched: a negative length counts as 0, row numbers are clipped
+ * to the rows there are, and a page that is not in the pool (or beyond the table's width) is never followed: see status.
+ * Slots at or past seqlens_k[b], and pages of which no row sees a key, may hold anything.
+ */
+typedef struct fa_paged_kv {
+    void* k;                  /* device, dtype: [num_pages, heads, page_size, head_dim], in any order of the first three */
+    void* v;                  /* like k; 16-byte aligned both */
+    int dtype;                /* FA_DTYPE_FP16 | FA_DTYPE_BF16 */
+    int num_pages;
+    int page_size;            /* a power of two, 8 or more */
+    int heads, head_dim;      /* K/V heads; head_dim a multiple of 8, <= 128 */
+    int64_t k_stride[3];      /* elements from one page, head and slot to the next; multiples of 8 */
+    int64_t v_stride[3];
+    const int* page_table;    /* device int32 [batch, table_width] */
+    int64_t table_stride;     /* elements from one sequence's row to the next */
+    int table_width;
+    int batch;
+    const int* seqlens_k;     /* device int32 [batch] */
+    const int* cu_seqlens_q;  /* device int32 [batch + 1], or NULL: one new token a sequence */
+} fa_paged_kv;
+
+/* Angles of the rotation: pair i of rotary_dim / 2 turns by inv_freq[i] a position, base^(-2 i / rotary_dim) where kind is
+ * FA_ROTARY_PLAIN.  For contexts longer than the model was trained on: FA_ROTARY_LINEAR divides every angle by factor;
+ * FA_ROTARY_NTK raises the base to base * factor^(rotary_dim / (rotary_dim - 2)); FA_ROTARY_RAMP divides by factor the pairs that
+ * make low_turns or fewer over original_length positions, keeps those that make high_turns or more, and goes over linearly between,
+ * with *amplitude = 0.1 ln factor + 1 (1 for the others).  Host arithmetic in 64 bits; inv_freq is a host buffer. */
+#define FA_ROTARY_PLAIN 0
+#define FA_ROTARY_LINEAR 1
+#define FA_ROTARY_NTK 2
+#define FA_ROTARY_RAMP 3
+int fa_rotary_frequencies(int rotary_dim, double base, int kind, double factor, double original_length, double low_turns,
+                          double high_turns, double* inv_freq, double* amplitude);
+
+/* y = the rows of x turned by their positions: with theta = position * inv_freq[i],
+ *   y[a] = amplitude (x[a] cos theta - x[b] sin theta),  y[b] = amplitude (x[b] cos theta + x[a] sin theta)
+ * for the columns (a, b) = (i, i + rotary_dim / 2), interleaved: (2 i, 2 i + 1); columns from rotary_dim on are copied.
+ * inverse: sin theta -> -sin theta, the transposed map, which takes the gradient of y to that of x.
+ * Angles are taken modulo a turn in 64-bit fixed point (exact to 2^-53 of a turn a position), sines, cosines and products are in
+ * 32 bits, the result is rounded once. */
+typedef struct fa_rotary_params {
+    const void* x;            /* device, dtype: [batch, heads, rows, head_dim], in any order of the first three */
+    void* y;                  /* device, dtype; x itself (with the same strides), or memory that does not overlap it */
+    int dtype;                /* FA_DTYPE_FP16 | FA_DTYPE_BF16 | FA_DTYPE_FP32 */
+    int batch, heads, rows, head_dim;
+    int rotary_dim;           /* even, <= head_dim */
+    int64_t x_stride[3];      /* elements from one batch, head and row to the next */
+    int64_t y_stride[3];
+    const void* positions;    /* device int32 or int64 [batch, rows] or [rows] */
+    int positions_64;         /* 1: they are int64 */
+    int64_t position_stride;  /* elements from one batch's positions to the next; 0: the same for all */
+    const double* inv_freq;   /* device fp64 [rotary_dim / 2] */
+    float amplitude;
+    int interleaved, inverse;
+    void* stream;
+} fa_rotary_params;
+int fa_rotary(const fa_rotary_params* p);
+
+/* Puts the new tokens' K and V into their slots, K (and, where q is given, Q into q_out) turned by the tokens' positions as fa_rotary
+ * does; without inv_freq nothing is turned and q must be NULL.  One launch. */
+typedef struct fa_paged_append_params {
+    fa_paged_kv cache;
+    const void* k;            /* device, cache.dtype: [tokens, cache.heads, head_dim] */
+    const void* v;
+    const void* q;            /* device, cache.dtype: [tokens, heads, head_dim], or NULL */
+    void* q_out;              /* like q; q itself (with the same strides), or memory that does not overlap it */
+    int64_t tokens;
+    int heads;                /* query heads */
+    int64_t k_new_stride[2];  /* elements from one token and head to the next */
+    int64_t v_new_stride[2];
+    int64_t q_stride[2];
+    int64_t q_out_stride[2];
+    int rotary_dim;           /* as in fa_rotary_params; 0 with inv_freq NULL */
+    const double* inv_freq;
+    float amplitude;
+    int interleaved;
+    int* status;              /* device int or NULL: FA_STATUS_PAGE where a token had no page of the pool to go to (it is dropped) */
+    void* stream;
+} fa_paged_append_params;
+int fa_paged_append(const fa_paged_append_params* p);
+
+/* Attention of the new tokens over their sequences' pages: causal, local, ALiBi as in fa_fwd, with the positions above; query head
+ * h reads K/V head h / (heads / cache.heads).  A row that sees no key gets O = 0, LSE = -inf. */
+typedef struct fa_paged_fwd_params {
+    fa_paged_kv cache;
+    const void* q;            /* device, cache.dtype: [tokens, heads, head_dim] */
+    void* o;                  /* device, o_dtype: like q */
+    float* lse;               /* device fp32 [tokens, heads], or NULL */
+    int o_dtype;              /* cache.dtype, or FA_DTYPE_FP32 */
+    int heads;                /* a multiple of cache.heads, at most 128 times it */
+    int64_t tokens;
+    int64_t q_stride[2];      /* elements from one token and head to the next; multiples of 8 */
+    int64_t o_stride[2];      /* multiples of 4 */
+    int max_seqlen_q;         /* most new tokens of a sequence: says which kernel suits, results do not depend on it */
+    float softmax_scale;      /* > 0 */
+    int is_causal;
+    int window_left, window_right;
+    const float* alibi_slopes;/* device fp32 [heads] or NULL */
+    void* workspace;          /* device, 16-byte aligned: partial results of sequences whose keys several CTAs share */
+    size_t workspace_bytes;   /* at least fa_paged_fwd_workspace_bytes(p) */
+    int* status;              /* device int or NULL.  FA_STATUS_PAGE: a visible key's page is not in the pool (the rows of the CTAs
+                                 that met it are NaN).  300 + n: a bounded wait gave up, as in fa_fwd_params: O and LSE are undefined. */
+    void* stream;
+} fa_paged_fwd_params;
+#define FA_STATUS_PAGE 400
+int fa_paged_fwd(const fa_paged_fwd_params* p);
+/* From the sizes alone: pointers are not followed, and lengths on the device do not count. */
+size_t fa_paged_fwd_workspace_bytes(const fa_paged_fwd_params* p);
+
 /* Message for a return code. */
 const char* fa_strerror(int code);
 int fa_version(void);
