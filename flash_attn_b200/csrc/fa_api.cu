@@ -358,6 +358,17 @@ int run_fwd(const fa_fwd_params* p, int o_dim, int splits, int sms) {
 
 int fa::current_device(int* sms, int* major) { return sm_count_of_current_device(sms, major); }
 
+int fa::encode_map(CUtensorMap* m, int dtype, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
+    const encode_tiled_fn enc = get_encode_tiled();
+    if (!enc) return FA_ERR_CUDA;
+    const cuuint32_t steps[5] = {1, 1, 1, 1, 1};
+    return enc(m, dtype == FA_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, static_cast<cuuint32_t>(rank),
+               const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? FA_OK
+               : FA_ERR_CUDA;
+}
+
 extern "C" {
 
 int fa_version(void) { return FA_B200_VERSION; }

@@ -1,112 +1,94 @@
-// Attention of new tokens over a paged K/V cache: the C entry point and its checks.
-//
-// One warp = one (row, head): 32 keys at a time, a lane each for the scores, then the lanes over the columns of V.
+// Attention of new tokens over a paged K/V cache: the C entry point, its checks and tensor maps, and the kernel that puts the parts of
+// split rows together.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
+#include <cstring>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include "fa_internal.h"
 #include "fa_paged.h"
+#include "paged_kernels.h"
+#include "paged_plan.cuh"
 #include "sm100_ptx.cuh"
 
 namespace fa {
 
 namespace {
 
-struct PagedArgs {
-    SeqTable seq;
-    const void *q, *k, *v;
-    void* o;
-    float* lse;
-    const int* page_table;
-    long long table_stride;
-    int table_width, num_pages, page_shift;
-    int heads, group, head_dim;
-    long long qs[2], os[2], ks[3], vs[3];
-    float scale;
-    int is_causal, window_left, window_right;
-    const float* alibi_slopes;
-    int o_is_fp32;
-    int* status;
-};
+// A part is not worth starting for fewer tiles than this, and shares above kLongShare are cut into waves.
+constexpr int kMinShare = 4, kLongShare = 24;
+constexpr int kCThreads = 128;
+constexpr int kCRows = 16;  // rows of a CTA of the combine kernel
 
-template <typename T> __device__ __forceinline__ float to_f(T x);
-template <> __device__ __forceinline__ float to_f<__half>(__half x) { return __half2float(x); }
-template <> __device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <typename T> __device__ __forceinline__ T from_f(float x);
-template <> __device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
-
-template <typename T>
-__global__ void __launch_bounds__(128) paged_rows_kernel(const PagedArgs a) {
+// One warp per row: O = sum_j 2^(m_j - m) O_j / l, l = sum_j 2^(m_j - m) l_j over the row's parts.  A CTA works the launch's plan out as
+// the kernel before it did, to find its item; it is resident and waiting when that kernel ends.
+template <int D, bool kBf16>
+__global__ void __launch_bounds__(kCThreads) paged_combine_kernel(const __grid_constant__ PagedArgs a) {
+    __shared__ PlanScratch<kCThreads> sm;
     grid_dep_launch_dependents();
-    __shared__ float q_row[4][128];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const long long item = static_cast<long long>(blockIdx.x) * 4 + warp;
-    const int token = static_cast<int>(item / a.heads), h = static_cast<int>(item - static_cast<long long>(token) * a.heads);
     grid_dep_wait();
-    if (token >= a.seq.tokens) return;
-    int b = -1;
-    SeqSpan s = {0, 0, 0};
-    for (int i = 0; i < a.seq.batch; ++i) {
-        s = seq_span(a.seq, i);
-        if (token >= s.first && token < s.end) { b = i; break; }
-    }
-    if (b < 0) return;
-    const long long pos = static_cast<long long>(s.keys) - s.end + token;
-    const int kh = h / a.group;
-    for (int c = lane; c < a.head_dim; c += 32) q_row[warp][c] = to_f(static_cast<const T*>(a.q)[token * a.qs[0] + h * a.qs[1] + c]);
-    __syncwarp();
-    const float slope = a.alibi_slopes ? a.alibi_slopes[h] : 0.0f;
-    float m = -INFINITY, l = 0.0f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    bool bad = false;
-    for (long long k0 = 0; k0 < s.keys; k0 += 32) {
-        const long long key = k0 + lane;
-        bool see = key < s.keys && (!a.is_causal || key <= pos) && (a.window_left < 0 || pos - key <= a.window_left) &&
-                   (a.window_right < 0 || key - pos <= a.window_right);
-        int page = -1;
-        float score = -INFINITY;
-        if (see) {
-            const long long nth = key >> a.page_shift;
-            if (nth < a.table_width) page = a.page_table[b * a.table_stride + nth];
-            if (page < 0 || page >= a.num_pages) { bad = true; see = false; }
+    PagedWork w;
+    if (!find_work<kCThreads>(a.plan, sm, static_cast<int>(blockIdx.x), true, &w) || w.parts == 1) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int row0 = w.blk * a.plan.rows;
+    const int n_rows = min(min(a.plan.rows, w.n * a.plan.group - row0), static_cast<int>(blockIdx.y + 1) * kCRows);
+    const bool mine = lane * 4 < D;
+    for (int n = blockIdx.y * kCRows + warp; n < n_rows; n += kCThreads / 32) {
+        const long long at0 = static_cast<long long>(w.slot) * a.plan.rows + n;  // part j's: + j * plan.rows
+        float m = -INFINITY, l = 0.0f;
+        for (int j = lane; j < w.parts; j += 32) m = fmaxf(m, a.ml_partial[at0 + static_cast<long long>(j) * a.plan.rows].x);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const float base = m == -INFINITY ? 0.0f : m;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int j0 = 0; j0 < w.parts; j0 += 32) {
+            float wt = 0.0f;
+            if (j0 + lane < w.parts) {
+                const float2 ml = a.ml_partial[at0 + static_cast<long long>(j0 + lane) * a.plan.rows];
+                wt = exp2f(ml.x - base);
+                l += ml.x == -INFINITY ? ml.y : wt * ml.y;  // (no key: l = 0; nothing but NaN: NaN)
+            }
+            const int n_parts = min(32, w.parts - j0);
+            for (int j = 0; j < n_parts; j += 8) {
+                float4 v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (mine && j + i < n_parts)
+                        v[i] = *reinterpret_cast<const float4*>(a.o_partial + (at0 + static_cast<long long>(j0 + j + i) * a.plan.rows) * D + lane * 4);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float x = __shfl_sync(0xffffffffu, wt, (j + i) & 31);
+                    if (mine && j + i < n_parts && x != 0.0f) {
+                        acc.x = fmaf(x, v[i].x, acc.x);
+                        acc.y = fmaf(x, v[i].y, acc.y);
+                        acc.z = fmaf(x, v[i].z, acc.z);
+                        acc.w = fmaf(x, v[i].w, acc.w);
+                    }
+                }
+            }
         }
-        const long long slot = key & ((1 << a.page_shift) - 1);
-        if (see) {
-            const T* kr = static_cast<const T*>(a.k) + page * a.ks[0] + kh * a.ks[1] + slot * a.ks[2];
-            float dot = 0.0f;
-            for (int c = 0; c < a.head_dim; ++c) dot = fmaf(q_row[warp][c], to_f(kr[c]), dot);
-            score = dot * a.scale - slope * fabsf(static_cast<float>(key - pos));
+#pragma unroll
+        for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // (NaN stays)
+        const int tok = static_cast<int>(fast_div(a.div_group, static_cast<uint32_t>(row0 + n)));
+        const int head = w.head * a.plan.group + row0 + n - tok * a.plan.group;
+        const long long token = w.first + tok;
+        if (lane * 4 < a.head_dim) {
+            const long long at = token * a.o_stride[0] + head * a.o_stride[1] + lane * 4;
+            const float4 o = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+            if (a.o_is_fp32) {
+                *reinterpret_cast<float4*>(static_cast<float*>(a.o) + at) = o;
+            } else if (kBf16) {
+                const __nv_bfloat162 x = __floats2bfloat162_rn(o.x, o.y), y = __floats2bfloat162_rn(o.z, o.w);
+                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + at) = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+            } else {
+                const __half2 x = __floats2half2_rn(o.x, o.y), y = __floats2half2_rn(o.z, o.w);
+                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + at) = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+            }
         }
-        float m_new = score;
-        for (int o = 16; o; o >>= 1) m_new = fmaxf(m_new, __shfl_xor_sync(0xffffffffu, m_new, o));
-        m_new = fmaxf(m, m_new);
-        const float base = m_new == -INFINITY ? 0.0f : m_new;
-        const float f = expf(m - base), p = expf(score - base);
-        m = m_new;
-        float sum = p;
-        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        l = l * f + sum;
-        for (int i = 0; i < 4; ++i) acc[i] *= f;
-        for (int j = 0; j < 32; ++j) {
-            if (!__shfl_sync(0xffffffffu, see ? 1 : 0, j)) continue;
-            const float pj = __shfl_sync(0xffffffffu, p, j);
-            const long long at = __shfl_sync(0xffffffffu, page, j) * a.vs[0] + kh * a.vs[1] + __shfl_sync(0xffffffffu, slot, j) * a.vs[2];
-            for (int i = 0; i < 4; ++i)
-                if (i * 32 + lane < a.head_dim) acc[i] = fmaf(pj, to_f(static_cast<const T*>(a.v)[at + i * 32 + lane]), acc[i]);
-        }
+        if (lane == 0 && a.lse != nullptr) a.lse[token * a.heads + head] = l == 0.0f ? -INFINITY : fmaf(m, 0.6931471805599453f, logf(l));
     }
-    bad = __any_sync(0xffffffffu, bad);
-    if (bad && lane == 0 && a.status) atomicExch(a.status, FA_STATUS_PAGE);
-    for (int i = 0; i < 4; ++i) {
-        const int c = i * 32 + lane;
-        if (c >= a.head_dim) continue;
-        const float x = bad ? __int_as_float(0x7fc00000) : l > 0.0f ? acc[i] / l : l == 0.0f ? 0.0f : l;
-        const long long at = token * a.os[0] + h * a.os[1] + c;
-        if (a.o_is_fp32) static_cast<float*>(a.o)[at] = x;
-        else static_cast<T*>(a.o)[at] = from_f<T>(x);
-    }
-    if (lane == 0 && a.lse) a.lse[static_cast<long long>(token) * a.heads + h] = bad ? __int_as_float(0x7fc00000) : l == 0.0f ? -INFINITY : m + logf(l);
 }
 
 int check_fwd(const fa_paged_fwd_params* p) {
@@ -133,7 +115,88 @@ int check_fwd(const fa_paged_fwd_params* p) {
     return FA_OK;
 }
 
+
+// What the sizes of a call say about its launch; the lengths, which say the rest, are on the device.
+struct PagedLaunch {
+    int columns;               // rows of a block
+    int wide;                  // columns of a partial row: head_dim rounded up
+    long long items;           // at most so many blocks of rows there are, over all K/V heads
+    long long grid, split_items, partials;
+    size_t o_bytes, bytes;     // workspace: partial rows, and all
+};
+
+PagedLaunch plan_launch(const fa_paged_fwd_params* p, int sms) {
+    const fa_paged_kv& c = p->cache;
+    PagedLaunch l = {};
+    const int group = p->heads / c.heads;
+    const long long rows = static_cast<long long>(std::min<int64_t>(p->max_seqlen_q, p->tokens)) * group;
+    l.columns = rows == 1 ? 1 : rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
+    l.wide = c.head_dim <= 64 ? 64 : 128;
+    l.items = c.heads * (c.cu_seqlens_q ? (p->tokens * group + static_cast<long long>(c.batch) * (l.columns - 1)) / l.columns
+                                        : static_cast<long long>(c.batch) * ((group + l.columns - 1) / l.columns));
+    const long long slots = 2LL * sms;
+    const long long tiles = (static_cast<long long>(c.table_width) * c.page_size + kTile - 1) / kTile;
+    const long long parts = (tiles + kMinShare - 1) / kMinShare;  // of one item
+    if (parts > 1) {
+        l.partials = std::min(most_partials(static_cast<int>(slots)), l.items * parts);
+        l.split_items = std::min(l.items, kPagedWaves * slots);
+    }
+    l.grid = l.items + (parts > 1 ? std::min(kPagedWaves * slots, l.items * (parts - 1)) : 0);
+    l.o_bytes = (static_cast<size_t>(l.partials) * l.columns * l.wide * sizeof(float) + 255) & ~static_cast<size_t>(255);
+    l.bytes = l.o_bytes + ((static_cast<size_t>(l.partials) * l.columns * sizeof(float2) + 255) & ~static_cast<size_t>(255));
+    return l;
+}
+
+// [pages, heads, slots, d] in any order of the first three, box = 64 columns x box_rows slots, 128-byte swizzle, zeros outside.  The last
+// maps are kept per host thread: they are a function of these arguments alone.
+int paged_map(CUtensorMap* m, const fa_paged_kv& c, const void* base, const int64_t* stride, int box_rows) {
+    struct Entry {
+        const void* base;
+        int64_t stride[3];
+        int dtype, pages, heads, page_size, d, box_rows;
+        bool valid;
+        CUtensorMap map;
+    };
+    constexpr int kEntries = 8;
+    thread_local Entry cache[kEntries] = {};
+    thread_local int next_victim = 0;
+    const int64_t counts[3] = {c.num_pages, c.heads, c.page_size};
+    int64_t s[3];
+    for (int i = 0; i < 3; ++i) s[i] = counts[i] > 1 ? stride[i] : 128;  // (of a dimension of one any stride will do)
+    for (const Entry& e : cache) {
+        if (e.valid && e.base == base && std::equal(s, s + 3, e.stride) && e.dtype == c.dtype && e.pages == c.num_pages && e.heads == c.heads &&
+            e.page_size == c.page_size && e.d == c.head_dim && e.box_rows == box_rows) {
+            *m = e.map;
+            return FA_OK;
+        }
+    }
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c.head_dim), static_cast<cuuint64_t>(c.page_size), static_cast<cuuint64_t>(c.heads),
+                                static_cast<cuuint64_t>(c.num_pages)};
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(s[2]) * 2, static_cast<cuuint64_t>(s[1]) * 2, static_cast<cuuint64_t>(s[0]) * 2};
+    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_rows), 1, 1};
+    const int rc = encode_map(m, c.dtype, 4, base, dims, strides, box);
+    if (rc != FA_OK) return rc;
+    Entry& e = cache[next_victim];
+    next_victim = (next_victim + 1) % kEntries;
+    e = {base, {s[0], s[1], s[2]}, c.dtype, c.num_pages, c.heads, c.page_size, c.head_dim, box_rows, true, *m};
+    return FA_OK;
+}
+
 }  // namespace
+
+cudaError_t launch_paged_combine(const PagedArgs& a, bool bf16, unsigned items, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(items, static_cast<unsigned>((a.plan.rows + kCRows - 1) / kCRows));
+    cfg.blockDim = dim3(kCThreads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (a.head_dim <= 64) return cudaLaunchKernelEx(&cfg, bf16 ? paged_combine_kernel<64, true> : paged_combine_kernel<64, false>, a);
+    return cudaLaunchKernelEx(&cfg, bf16 ? paged_combine_kernel<128, true> : paged_combine_kernel<128, false>, a);
+}
 
 }  // namespace fa
 
@@ -141,7 +204,12 @@ using namespace fa;
 
 extern "C" {
 
-size_t fa_paged_fwd_workspace_bytes(const fa_paged_fwd_params* p) { return check_fwd(p) == FA_OK ? 0 : 0; }
+size_t fa_paged_fwd_workspace_bytes(const fa_paged_fwd_params* p) {
+    if (check_fwd(p) != FA_OK) return 0;
+    int sms = 148, major = 10;
+    if (current_device(&sms, &major) != FA_OK) sms = 148;
+    return plan_launch(p, sms).bytes;
+}
 
 int fa_paged_fwd(const fa_paged_fwd_params* p) {
     int rc = check_fwd(p);
@@ -149,12 +217,25 @@ int fa_paged_fwd(const fa_paged_fwd_params* p) {
     int sms = 0, major = 0;
     if ((rc = current_device(&sms, &major)) != FA_OK) return rc;
     if (major != 10) return FA_ERR_NOT_SM100;
+    const PagedLaunch l = plan_launch(p, sms);
+    if (l.grid > 0x7fffffffLL) return FA_ERR_TOO_LARGE;
+    if (l.bytes > 0 && (!p->workspace || p->workspace_bytes < l.bytes)) return FA_ERR_WORKSPACE;
+    if (l.bytes > 0 && (reinterpret_cast<uintptr_t>(p->workspace) & 15u)) return FA_ERR_INVALID_ARG;
     const fa_paged_kv& c = p->cache;
     PagedArgs a = {};
-    a.seq = {c.seqlens_k, c.cu_seqlens_q, c.batch, static_cast<int>(p->tokens)};
+    a.plan.seq = {c.seqlens_k, c.cu_seqlens_q, c.batch, static_cast<int>(p->tokens)};
+    a.plan.heads_k = c.heads;
+    a.plan.group = p->heads / c.heads;
+    a.plan.rows = l.columns;
+    a.plan.is_causal = p->is_causal ? 1 : 0;
+    a.plan.window_left = p->window_left;
+    a.plan.window_right = p->window_right;
+    a.plan.slots = 2 * sms;
+    a.plan.min_share = kMinShare;
+    a.plan.long_share = kLongShare;
+    a.plan.partials = static_cast<int>(l.partials);
+    a.div_group = make_fastdiv(static_cast<uint32_t>(a.plan.group));
     a.q = p->q;
-    a.k = c.k;
-    a.v = c.v;
     a.o = p->o;
     a.lse = p->lse;
     a.page_table = c.page_table;
@@ -163,32 +244,26 @@ int fa_paged_fwd(const fa_paged_fwd_params* p) {
     a.num_pages = c.num_pages;
     while ((1 << a.page_shift) < c.page_size) ++a.page_shift;
     a.heads = p->heads;
-    a.group = p->heads / c.heads;
     a.head_dim = c.head_dim;
-    std::copy(p->q_stride, p->q_stride + 2, a.qs);
-    std::copy(p->o_stride, p->o_stride + 2, a.os);
-    std::copy(c.k_stride, c.k_stride + 3, a.ks);
-    std::copy(c.v_stride, c.v_stride + 3, a.vs);
-    a.scale = p->softmax_scale;
-    a.is_causal = p->is_causal;
-    a.window_left = p->window_left;
-    a.window_right = p->window_right;
+    std::copy(p->q_stride, p->q_stride + 2, a.q_stride);
+    std::copy(p->o_stride, p->o_stride + 2, a.o_stride);
+    a.scale_log2 = p->softmax_scale * 1.4426950408889634f;
     a.alibi_slopes = p->alibi_slopes;
     a.o_is_fp32 = p->o_dtype == FA_DTYPE_FP32;
     a.status = p->status;
-    const long long rows = p->tokens * p->heads;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>((rows + 3) / 4));
-    cfg.blockDim = dim3(128);
-    cfg.stream = static_cast<cudaStream_t>(p->stream);
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    const cudaError_t e = c.dtype == FA_DTYPE_BF16 ? cudaLaunchKernelEx(&cfg, paged_rows_kernel<__nv_bfloat16>, a)
-                                                   : cudaLaunchKernelEx(&cfg, paged_rows_kernel<__half>, a);
-    return e == cudaSuccess ? FA_OK : FA_ERR_CUDA;
+    if (l.bytes > 0) {
+        a.o_partial = static_cast<float*>(p->workspace);
+        a.ml_partial = reinterpret_cast<float2*>(static_cast<char*>(p->workspace) + l.o_bytes);
+    }
+    CUtensorMap tk, tv;
+    const int box_rows = std::min(c.page_size, kTile);
+    if ((rc = paged_map(&tk, c, c.k, c.k_stride, box_rows)) != FA_OK) return rc;
+    if ((rc = paged_map(&tv, c, c.v, c.v_stride, box_rows)) != FA_OK) return rc;
+    cudaStream_t stream = static_cast<cudaStream_t>(p->stream);
+    const bool bf16 = c.dtype == FA_DTYPE_BF16;
+    if (launch_paged_decode(a, tk, tv, l.columns, bf16, static_cast<unsigned>(l.grid), stream) != cudaSuccess) return FA_ERR_CUDA;
+    if (l.partials > 0 && launch_paged_combine(a, bf16, static_cast<unsigned>(l.split_items), stream) != cudaSuccess) return FA_ERR_CUDA;
+    return FA_OK;
 }
 
 }  // extern "C"

@@ -1,6 +1,7 @@
 // What the kernels around the paged K/V cache share: its device-side description, and where a new token stands.
 #pragma once
 #include <cstdint>
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include "../../include/fa_b200.h"
 
@@ -8,6 +9,8 @@ namespace fa {
 
 // (SM count and compute capability of the current device, kept per device: fa_api.cu)
 int current_device(int* sms, int* major);
+// A tensor map of 16-bit elements, boxes with the 128-byte swizzle; out-of-range elements read as zero.  (fa_api.cu)
+int encode_map(CUtensorMap* m, int dtype, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box);
 // Whether rows of `columns` elements with these counts and strides (of up to three dimensions) lie apart from each other, one
 // dimension inside another: what is written must.
 bool rows_apart(const int64_t* counts, const int64_t* strides, int n, int64_t columns);
