@@ -118,7 +118,10 @@ int check_fwd(const fa_paged_fwd_params* p) {
 
 // What the sizes of a call say about its launch; the lengths, which say the rest, are on the device.
 struct PagedLaunch {
-    int columns;               // rows of a block
+    int columns;               // decode kernel: rows of a block; 0: the tiled kernel
+    int query_tiles;           // tiled kernel: of a block
+    int rows;                  // of a block
+    int slots;                 // CTAs that run at once
     int wide;                  // columns of a partial row: head_dim rounded up
     long long items;           // at most so many blocks of rows there are, over all K/V heads
     long long grid, split_items, partials;
@@ -130,11 +133,15 @@ PagedLaunch plan_launch(const fa_paged_fwd_params* p, int sms) {
     PagedLaunch l = {};
     const int group = p->heads / c.heads;
     const long long rows = static_cast<long long>(std::min<int64_t>(p->max_seqlen_q, p->tokens)) * group;
-    l.columns = rows == 1 ? 1 : rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
+    const int tile_rows = kTile / group * group;
+    l.columns = rows == 1 ? 1 : rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 ? 16 : 0;
+    l.query_tiles = l.columns ? 0 : rows <= tile_rows ? 1 : 2;
+    l.rows = l.columns ? l.columns : l.query_tiles * tile_rows;
+    l.slots = (l.query_tiles == 2 ? 1 : 2) * sms;
     l.wide = c.head_dim <= 64 ? 64 : 128;
-    l.items = c.heads * (c.cu_seqlens_q ? (p->tokens * group + static_cast<long long>(c.batch) * (l.columns - 1)) / l.columns
-                                        : static_cast<long long>(c.batch) * ((group + l.columns - 1) / l.columns));
-    const long long slots = 2LL * sms;
+    l.items = c.heads * (c.cu_seqlens_q ? (p->tokens * group + static_cast<long long>(c.batch) * (l.rows - 1)) / l.rows
+                                        : static_cast<long long>(c.batch) * ((group + l.rows - 1) / l.rows));
+    const long long slots = l.slots;
     const long long tiles = (static_cast<long long>(c.table_width) * c.page_size + kTile - 1) / kTile;
     const long long parts = (tiles + kMinShare - 1) / kMinShare;  // of one item
     if (parts > 1) {
@@ -142,44 +149,63 @@ PagedLaunch plan_launch(const fa_paged_fwd_params* p, int sms) {
         l.split_items = std::min(l.items, kPagedWaves * slots);
     }
     l.grid = l.items + (parts > 1 ? std::min(kPagedWaves * slots, l.items * (parts - 1)) : 0);
-    l.o_bytes = (static_cast<size_t>(l.partials) * l.columns * l.wide * sizeof(float) + 255) & ~static_cast<size_t>(255);
-    l.bytes = l.o_bytes + ((static_cast<size_t>(l.partials) * l.columns * sizeof(float2) + 255) & ~static_cast<size_t>(255));
+    l.o_bytes = (static_cast<size_t>(l.partials) * l.rows * l.wide * sizeof(float) + 255) & ~static_cast<size_t>(255);
+    l.bytes = l.o_bytes + ((static_cast<size_t>(l.partials) * l.rows * sizeof(float2) + 255) & ~static_cast<size_t>(255));
     return l;
 }
 
-// [pages, heads, slots, d] in any order of the first three, box = 64 columns x box_rows slots, 128-byte swizzle, zeros outside.  The last
-// maps are kept per host thread: they are a function of these arguments alone.
-int paged_map(CUtensorMap* m, const fa_paged_kv& c, const void* base, const int64_t* stride, int box_rows) {
+// A 4-D tensor map: dims and strides (elements; of a dimension of one any will do) outermost last.  The last ones are kept per host
+// thread, being a function of these arguments alone.
+int map_of(CUtensorMap* m, int dtype, const void* base, const int64_t (&dims)[4], const int64_t (&strides)[3], const int (&box)[4]) {
     struct Entry {
         const void* base;
-        int64_t stride[3];
-        int dtype, pages, heads, page_size, d, box_rows;
+        int64_t dims[4], strides[3];
+        int box[4], dtype;
         bool valid;
         CUtensorMap map;
     };
-    constexpr int kEntries = 8;
+    constexpr int kEntries = 12;
     thread_local Entry cache[kEntries] = {};
     thread_local int next_victim = 0;
-    const int64_t counts[3] = {c.num_pages, c.heads, c.page_size};
-    int64_t s[3];
-    for (int i = 0; i < 3; ++i) s[i] = counts[i] > 1 ? stride[i] : 128;  // (of a dimension of one any stride will do)
     for (const Entry& e : cache) {
-        if (e.valid && e.base == base && std::equal(s, s + 3, e.stride) && e.dtype == c.dtype && e.pages == c.num_pages && e.heads == c.heads &&
-            e.page_size == c.page_size && e.d == c.head_dim && e.box_rows == box_rows) {
+        if (e.valid && e.base == base && e.dtype == dtype && std::equal(dims, dims + 4, e.dims) && std::equal(strides, strides + 3, e.strides) &&
+            std::equal(box, box + 4, e.box)) {
             *m = e.map;
             return FA_OK;
         }
     }
-    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c.head_dim), static_cast<cuuint64_t>(c.page_size), static_cast<cuuint64_t>(c.heads),
-                                static_cast<cuuint64_t>(c.num_pages)};
-    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(s[2]) * 2, static_cast<cuuint64_t>(s[1]) * 2, static_cast<cuuint64_t>(s[0]) * 2};
-    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_rows), 1, 1};
-    const int rc = encode_map(m, c.dtype, 4, base, dims, strides, box);
+    cuuint64_t d[4], s[3];
+    cuuint32_t b[4];
+    for (int i = 0; i < 4; ++i) {
+        d[i] = static_cast<cuuint64_t>(dims[i]);
+        b[i] = static_cast<cuuint32_t>(box[i]);
+        if (i > 0) s[i - 1] = dims[i] > 1 ? static_cast<cuuint64_t>(strides[i - 1]) * 2 : 256;
+    }
+    const int rc = encode_map(m, dtype, 4, base, d, s, b);
     if (rc != FA_OK) return rc;
     Entry& e = cache[next_victim];
     next_victim = (next_victim + 1) % kEntries;
-    e = {base, {s[0], s[1], s[2]}, c.dtype, c.num_pages, c.heads, c.page_size, c.head_dim, box_rows, true, *m};
+    e.base = base;
+    std::copy(dims, dims + 4, e.dims);
+    std::copy(strides, strides + 3, e.strides);
+    std::copy(box, box + 4, e.box);
+    e.dtype = dtype;
+    e.map = *m;
+    e.valid = true;
     return FA_OK;
+}
+
+// Pages: a box is 64 columns of the tokens of a page (of 128 of them at most) of one head.
+int page_map(CUtensorMap* m, const fa_paged_kv& c, const void* base, const int64_t* stride) {
+    return map_of(m, c.dtype, base, {c.head_dim, c.page_size, c.heads, c.num_pages}, {stride[2], stride[1], stride[0]},
+                  {64, std::min(c.page_size, kTile), 1, 1});
+}
+
+// Q: a box is 64 columns of the rows of a query tile, the heads of one K/V head side by side.
+int query_map(CUtensorMap* m, const fa_paged_fwd_params* p) {
+    const int group = p->heads / p->cache.heads;
+    return map_of(m, p->cache.dtype, p->q, {p->cache.head_dim, group, p->cache.heads, p->tokens}, {p->q_stride[1], p->q_stride[1] * group, p->q_stride[0]},
+                  {64, group, 1, kTile / group});
 }
 
 }  // namespace
@@ -226,11 +252,11 @@ int fa_paged_fwd(const fa_paged_fwd_params* p) {
     a.plan.seq = {c.seqlens_k, c.cu_seqlens_q, c.batch, static_cast<int>(p->tokens)};
     a.plan.heads_k = c.heads;
     a.plan.group = p->heads / c.heads;
-    a.plan.rows = l.columns;
+    a.plan.rows = l.rows;
     a.plan.is_causal = p->is_causal ? 1 : 0;
     a.plan.window_left = p->window_left;
     a.plan.window_right = p->window_right;
-    a.plan.slots = 2 * sms;
+    a.plan.slots = l.slots;
     a.plan.min_share = kMinShare;
     a.plan.long_share = kLongShare;
     a.plan.partials = static_cast<int>(l.partials);
@@ -245,6 +271,7 @@ int fa_paged_fwd(const fa_paged_fwd_params* p) {
     while ((1 << a.page_shift) < c.page_size) ++a.page_shift;
     a.heads = p->heads;
     a.head_dim = c.head_dim;
+    a.tile_tokens = kTile / a.plan.group;
     std::copy(p->q_stride, p->q_stride + 2, a.q_stride);
     std::copy(p->o_stride, p->o_stride + 2, a.o_stride);
     a.scale_log2 = p->softmax_scale * 1.4426950408889634f;
@@ -256,12 +283,21 @@ int fa_paged_fwd(const fa_paged_fwd_params* p) {
         a.ml_partial = reinterpret_cast<float2*>(static_cast<char*>(p->workspace) + l.o_bytes);
     }
     CUtensorMap tk, tv;
-    const int box_rows = std::min(c.page_size, kTile);
-    if ((rc = paged_map(&tk, c, c.k, c.k_stride, box_rows)) != FA_OK) return rc;
-    if ((rc = paged_map(&tv, c, c.v, c.v_stride, box_rows)) != FA_OK) return rc;
+    if ((rc = page_map(&tk, c, c.k, c.k_stride)) != FA_OK) return rc;
+    if ((rc = page_map(&tv, c, c.v, c.v_stride)) != FA_OK) return rc;
     cudaStream_t stream = static_cast<cudaStream_t>(p->stream);
     const bool bf16 = c.dtype == FA_DTYPE_BF16;
-    if (launch_paged_decode(a, tk, tv, l.columns, bf16, static_cast<unsigned>(l.grid), stream) != cudaSuccess) return FA_ERR_CUDA;
+    const unsigned grid = static_cast<unsigned>(l.grid);
+    cudaError_t e;
+    if (l.columns) {
+        e = launch_paged_decode(a, tk, tv, l.columns, bf16, grid, stream);
+    } else {
+        CUtensorMap tq;
+        if ((rc = query_map(&tq, p)) != FA_OK) return rc;
+        if (l.wide == 64) e = l.query_tiles == 1 ? launch_paged_tiled<64, 1>(a, tq, tk, tv, bf16, grid, stream) : launch_paged_tiled<64, 2>(a, tq, tk, tv, bf16, grid, stream);
+        else e = l.query_tiles == 1 ? launch_paged_tiled<128, 1>(a, tq, tk, tv, bf16, grid, stream) : launch_paged_tiled<128, 2>(a, tq, tk, tv, bf16, grid, stream);
+    }
+    if (e != cudaSuccess) return FA_ERR_CUDA;
     if (l.partials > 0 && launch_paged_combine(a, bf16, static_cast<unsigned>(l.split_items), stream) != cudaSuccess) return FA_ERR_CUDA;
     return FA_OK;
 }

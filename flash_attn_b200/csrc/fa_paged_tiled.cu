@@ -1,0 +1,570 @@
+// Attention of chunks of new tokens over a paged K/V cache: tensor-bound.
+//
+// One CTA = one part of the keys of one block of rows (paged_plan.cuh), NQ query tiles of 128 rows.  A row is a token and a query head:
+// the heads of a K/V head lie side by side in a tile (row = token * group + head, as one TMA box of Q lands), so that they share every
+// K/V tile and a few tokens fill it; where the group does not divide 128 the tile's last rows are left over.
+// The walk is the tiled kernel's for contiguous K/V: a TMA warp feeds a ring of K/V tiles, an MMA warp issues S = Q K^T into tensor
+// memory, four softmax warps a query tile keep a row a thread, write P over S, and the MMA warp adds P V; two query tiles alternate
+// on the tensor pipe.  A KV tile is 128 / page_size pages (or a part of one), a box each, looked up and issued by a lane each.
+// KV tiles are visited from the last to the first: with a causal mask the second query tile's own diagonal tile comes first.
+//
+// What the pool holds beyond a sequence is not known, and 0 * NaN is NaN: rows of a V tile that no row of the block sees are
+// overwritten with zeros before its MMAs (first and last tile only).
+#include <algorithm>
+#include <atomic>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <type_traits>
+#include "paged_kernels.h"
+#include "paged_plan.cuh"
+#include "sm100_ptx.cuh"
+#include "tiled_mma.cuh"
+
+// (compiled once for each, side by side)
+#if !defined(FA_PAGED_D) || !defined(FA_PAGED_NQ)
+#error "compiled with FA_PAGED_D = 64 or 128 and FA_PAGED_NQ = 1 or 2"
+#endif
+
+namespace fa {
+
+namespace {
+
+constexpr float kRescaleThreshold = 8.0f;  // log2 units: rescale O only when the max grew by > 2^8
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// Column pairs that take the polynomial exp2, a quarter of them (see the tiled kernel for contiguous K/V).
+__host__ __device__ constexpr uint32_t poly_mask(int d, bool alibi) { return alibi ? 0x11u : d == 128 ? 0x88u : 0x81u; }
+
+template <int D, int NQ>
+struct TCfg {
+    static constexpr int kThreads = NQ == 2 ? 384 : 256;
+    // Registers: the CTA owns kThreads * kRegsLaunch from launch on (168 a thread under __launch_bounds__(384, 1), 128 under (256, 2));
+    // an increase that asks for more than the helper warps released would wait for ever.
+    static constexpr int kRegsLaunch = NQ == 2 ? 168 : 128;
+    static constexpr int kRegsHelper = NQ == 2 ? 56 : 48;
+    static constexpr int kRegsSoftmax = NQ == 2 ? 224 : 208;
+    static_assert(NQ * 128 * kRegsSoftmax + 128 * kRegsHelper <= kThreads * kRegsLaunch, "register hand-over exceeds the CTA's allocation");
+    static constexpr int kProducerWarp = NQ * 4, kMmaWarp = NQ * 4 + 1;
+    static constexpr int kStages = (D == 64) ? (NQ == 2 ? 3 : 2) : (NQ == 2 ? 2 : 1);
+    static constexpr int kBoxes = D / 64;
+    static constexpr int kTileBytes = kTile * D * 2;
+    static constexpr int kTmemCols = NQ == 2 ? 512 : 256;  // S_i at i * 128 (P_i over its first half), O_i behind them
+    static constexpr int kTmemO = NQ * kTile;
+    static constexpr int kSmemQ = 0;
+    static constexpr int kSmemK = NQ * kTileBytes;
+    static constexpr int kSmemV = kSmemK + kStages * kTileBytes;
+    static constexpr int kSmemBar = kSmemV + kStages * kTileBytes;
+    static constexpr int kNumBars = 1 + 2 * NQ + 4 * kStages;
+    static constexpr int kSmemMisc = kSmemBar + 8 * kNumBars;  // tensor-memory address, abort flag, bad page
+    static constexpr int kSmemPlan = (kSmemMisc + 16 + 15) / 16 * 16;
+    static constexpr int kSmemBytes = kSmemPlan + static_cast<int>(sizeof(PlanScratch<kThreads>)) + 1024;  // + alignment slack
+    static_assert(kSmemBytes <= (NQ == 2 ? 232448 : 115712), "one or two CTAs per SM");
+};
+
+template <int D, int NQ, bool kBf16, bool kAlibi>
+__global__ void __launch_bounds__(TCfg<D, NQ>::kThreads, NQ == 1 ? 2 : 1)
+paged_tiled_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+                   const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ PagedArgs a) {
+    using C = TCfg<D, NQ>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
+    const uint32_t sQ = smem_base + C::kSmemQ, sK = smem_base + C::kSmemK, sV = smem_base + C::kSmemV, bar0 = smem_base + C::kSmemBar;
+    const uint32_t bar_q_full = bar0;
+    const uint32_t bar_s_full = bar0 + 8;                      // [NQ]
+    const uint32_t bar_o_full = bar_s_full + 8 * NQ;           // [NQ]
+    const uint32_t bar_k_full = bar_o_full + 8 * NQ;           // [kStages]
+    const uint32_t bar_k_empty = bar_k_full + 8 * C::kStages;  // [kStages]
+    const uint32_t bar_v_full = bar_k_empty + 8 * C::kStages;  // [kStages]
+    const uint32_t bar_v_empty = bar_v_full + 8 * C::kStages;  // [kStages]
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem_gen + C::kSmemMisc);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem_gen + C::kSmemMisc + 4);
+    volatile int* bad_page = reinterpret_cast<volatile int*>(smem_gen + C::kSmemMisc + 8);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    grid_dep_launch_dependents();
+    if (warp == C::kProducerWarp) {
+        if (lane < C::kNumBars) mbar_init(bar0 + 8 * lane, 1);
+        if (lane == 0) {
+            *abort_flag = 0;
+            *bad_page = 0;
+            tma_prefetch_desc(&tmap_q);
+            tma_prefetch_desc(&tmap_k);
+            tma_prefetch_desc(&tmap_v);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_fence_init();
+    }
+    grid_dep_wait();  // every thread, before its first global access
+    PagedWork w;
+    if (!find_work<C::kThreads>(a.plan, *reinterpret_cast<PlanScratch<C::kThreads>*>(smem_gen + C::kSmemPlan), static_cast<int>(blockIdx.x), false, &w))
+        return;
+
+    // ---- the block's query tiles, and the tiles of keys of this part
+    const int tile_tokens = a.tile_tokens, tile_rows = tile_tokens * a.plan.group;
+    const int token0 = w.blk * NQ * tile_tokens;  // first token of the block inside the sequence
+    const int p_first = w.keys - w.n;             // position of the sequence's first new token
+    struct Range { int lo, hi; } range[NQ];
+    int vis_lo = 0x7fffffff, vis_hi = 0, lo = 0x7fffffff, hi = 0;
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+        const int t0 = token0 + i * tile_tokens, t1 = min(t0 + tile_tokens, w.n) - 1;
+        int l = 0, h = 0;
+        if (t1 >= t0) visible_keys(a.plan, w.keys, p_first + t0, p_first + t1, &l, &h);
+        range[i] = {l / kTile, h > l ? (h + kTile - 1) / kTile : l / kTile};
+        if (h > l) {
+            vis_lo = min(vis_lo, l);
+            vis_hi = max(vis_hi, h);
+            lo = min(lo, range[i].lo);
+            hi = max(hi, range[i].hi);
+        }
+    }
+    const int n_all = hi > lo ? hi - lo : 0, lo_all = hi > lo ? lo : 0;
+    if (w.parts > 1) {
+        const int p_lo = lo_all + static_cast<int>(static_cast<long long>(n_all) * w.part / w.parts);
+        const int p_hi = lo_all + static_cast<int>(static_cast<long long>(n_all) * (w.part + 1) / w.parts);
+        lo = 0x7fffffff;
+        hi = 0;
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+            range[i].lo = max(range[i].lo, p_lo);
+            range[i].hi = max(min(range[i].hi, p_hi), range[i].lo);
+            if (range[i].hi > range[i].lo) {
+                lo = min(lo, range[i].lo);
+                hi = max(hi, range[i].hi);
+            }
+        }
+    }
+    const int n_union = hi > lo ? hi - lo : 0;  // KV tiles of this CTA: [lo, hi)
+
+    // ---- set-up: loads of Q and the first K/V tiles, tensor memory
+    const int page_rows = min(1 << a.page_shift, kTile);  // tokens of a box
+    const int tile_pages = kTile / page_rows;
+    const int my_page = lane / C::kBoxes, my_box = lane % C::kBoxes;
+    const int* table = a.page_table + w.b * a.table_stride;
+    bool met_bad = false;
+    auto lookup = [&](int tile) -> int {  // the page that this lane loads, -1: none (no row of the block sees a key of it)
+        const int key = tile * kTile + my_page * page_rows;
+        if (my_page >= tile_pages || key >= vis_hi || key + page_rows <= vis_lo) return -1;
+        const int nth = key >> a.page_shift;
+        const int page = nth < a.table_width ? __ldg(table + nth) : -1;
+        if (page >= 0 && page < a.num_pages) return page;
+        met_bad = true;
+        return a.num_pages;  // outside of the tensor map: the box is zeros
+    };
+    auto load = [&](const CUtensorMap* map, uint32_t dst, uint32_t bar, int tile, int page) {
+        const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, page >= 0));
+        if (__any_sync(0xffffffffu, met_bad) && lane == 0) *bad_page = 1;  // (before what the readers' barriers wait for)
+        if (lane == 0) mbar_expect_tx(bar, boxes * page_rows * 128);
+        __syncwarp();
+        if (page >= 0)
+            tma_load_4d(dst + my_box * (kTile * 128) + my_page * (page_rows * 128), map, bar, my_box * 64,
+                        (tile * kTile) & ((1 << a.page_shift) - 1), w.head, page);
+    };
+    int prefilled = 0;
+    if (warp == C::kProducerWarp && n_union > 0) {
+        int page[C::kStages];
+        prefilled = min(C::kStages, n_union);
+#pragma unroll
+        for (int t = 0; t < C::kStages; ++t) page[t] = t < prefilled ? lookup(hi - 1 - t) : -1;
+        int q_tiles = 0;
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) q_tiles += token0 + i * tile_tokens < w.n ? 1 : 0;
+        if (lane == 0) mbar_expect_tx(bar_q_full, q_tiles * C::kBoxes * tile_rows * 128);
+        __syncwarp();
+        if (lane < q_tiles * C::kBoxes) {
+            const int i = lane / C::kBoxes, b = lane % C::kBoxes;
+            tma_load_4d(sQ + i * C::kTileBytes + b * (kTile * 128), &tmap_q, bar_q_full, b * 64, 0, w.head, w.first + token0 + i * tile_tokens);
+        }
+#pragma unroll
+        for (int t = 0; t < C::kStages; ++t) {  // KV tiles are walked from the last to the first
+            if (t >= prefilled) break;
+            load(&tmap_k, sK + t * C::kTileBytes, bar_k_full + 8 * t, hi - 1 - t, page[t]);
+            load(&tmap_v, sV + t * C::kTileBytes, bar_v_full + 8 * t, hi - 1 - t, page[t]);
+        }
+    }
+    if (warp == C::kMmaWarp && n_union > 0) {
+        tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), C::kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem_base = (n_union > 0) ? *tmem_slot : 0u;
+
+    int fail = 0;
+    if (warp >= NQ * 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsHelper));
+        if (n_union > 0 && warp == C::kProducerWarp) {
+            // ======================= TMA producer ===================================
+            for (int t = prefilled; t < n_union; ++t) {
+                const int st = t % C::kStages;
+                const uint32_t ph = (t / C::kStages) & 1;
+                const int tile = hi - 1 - t, page = lookup(tile);
+                if (!mbar_wait_warp(bar_k_empty + 8 * st, ph ^ 1, abort_flag)) { fail = 1; break; }
+                load(&tmap_k, sK + st * C::kTileBytes, bar_k_full + 8 * st, tile, page);
+                if (!mbar_wait_warp(bar_v_empty + 8 * st, ph ^ 1, abort_flag)) { fail = 2; break; }
+                load(&tmap_v, sV + st * C::kTileBytes, bar_v_full + 8 * st, tile, page);
+            }
+            if (__any_sync(0xffffffffu, met_bad) && lane == 0 && a.status != nullptr) atomicExch(a.status, FA_STATUS_PAGE);
+        } else if (n_union > 0 && warp == C::kMmaWarp) {
+            // ======================= MMA issuer =====================================
+            const bool leader = elect_one();
+            constexpr uint32_t idesc_qk = make_idesc_f16(kTile, kTile, kBf16, false);
+            constexpr uint32_t idesc_pv = make_idesc_f16(kTile, D, kBf16, true);
+            const uint64_t dqk = make_smem_desc(0, 0, 1024);
+            const uint64_t dvv = make_smem_desc(0, kTile * 128, 1024);
+            const uint32_t desc_hi = static_cast<uint32_t>(dqk >> 32);
+            const uint32_t q_lo = static_cast<uint32_t>(dqk) | (sQ >> 4), k_lo = static_cast<uint32_t>(dqk) | (sK >> 4), v_lo = static_cast<uint32_t>(dvv) | (sV >> 4);
+            auto issue_qk = [&](int i, int st) {
+                issue_qk_block<D>(tmem_base + i * kTile, q_lo + ((i * C::kTileBytes) >> 4), k_lo + ((st * C::kTileBytes) >> 4), desc_hi, idesc_qk);
+            };
+            auto active = [&](int i, int tile) { return tile >= range[i].lo && tile < range[i].hi; };
+            do {
+                if (!mbar_wait_warp(bar_q_full, 0, abort_flag)) { fail = 3; break; }
+                if (!mbar_wait_warp(bar_k_full, 0, abort_flag)) { fail = 4; break; }
+                tc_fence_after_sync();
+                if (leader) {
+#pragma unroll
+                    for (int i = 0; i < NQ; ++i) {
+                        if (active(i, hi - 1)) {
+                            issue_qk(i, 0);
+                            umma_commit(bar_s_full + 8 * i);
+                        }
+                    }
+                    umma_commit(bar_k_empty);
+                }
+                for (int t = 0; t < n_union && fail == 0; ++t) {
+                    const int tile = hi - 1 - t;
+                    const int st = t % C::kStages;
+                    const uint32_t ph = (t / C::kStages) & 1;
+                    const int st1 = (t + 1) % C::kStages;
+                    const uint32_t ph1 = ((t + 1) / C::kStages) & 1;
+                    const bool more = t + 1 < n_union;
+                    if (!mbar_wait_warp(bar_v_full + 8 * st, ph, abort_flag)) { fail = 6; break; }
+                    if (tile * kTile < vis_lo || tile * kTile + kTile > vis_hi) {
+                        // keys that no row of the block sees: their rows of V may hold anything
+                        const int head = max(vis_lo - tile * kTile, 0), tail = min(vis_hi - tile * kTile, kTile);
+                        const uint32_t v = sV + st * C::kTileBytes;
+                        for (int j = lane; j < kTile * C::kBoxes * 8; j += 32) {
+                            const int row = (j >> 3) % kTile;
+                            if (row < head || row >= tail) st_shared_v4(v + j * 16, 0u, 0u, 0u, 0u);
+                        }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                    if (more) {
+                        if (!mbar_wait_warp(bar_k_full + 8 * st1, ph1, abort_flag)) { fail = 7; break; }
+                    }
+#pragma unroll
+                    for (int i = 0; i < NQ; ++i) {
+                        if (active(i, tile)) {
+                            // P V starts on the first half of P while the second half is exponentiated
+                            named_sync(1 + 2 * i);
+                            tc_fence_after_sync();
+                            if (leader)
+                                issue_pv_first(tmem_base + C::kTmemO + i * D, tmem_base + i * kTile, v_lo + ((st * C::kTileBytes) >> 4), desc_hi, idesc_pv,
+                                               tile < range[i].hi - 1 ? 1u : 0u);
+                            named_sync(2 + 2 * i);
+                            tc_fence_after_sync();
+                            if (leader) {
+                                issue_pv_rest(tmem_base + C::kTmemO + i * D, tmem_base + i * kTile, v_lo + ((st * C::kTileBytes) >> 4), desc_hi, idesc_pv);
+                                if (tile == range[i].lo) umma_commit(bar_o_full + 8 * i);
+                            }
+                        }
+                        if (more && active(i, tile - 1)) {
+                            if (leader) {
+                                issue_qk(i, st1);
+                                umma_commit(bar_s_full + 8 * i);
+                            }
+                        }
+                    }
+                    if (leader) {
+                        umma_commit(bar_v_empty + 8 * st);
+                        if (more) umma_commit(bar_k_empty + 8 * st1);
+                    }
+                }
+            } while (false);
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kRegsSoftmax));
+        // ======================= softmax / epilogue =============================
+        const int qi = warp >> 2;           // which query tile of the CTA
+        const int r = threadIdx.x & 127;    // row inside the tile
+        const int r_tok = static_cast<int>(fast_div(a.div_group, static_cast<uint32_t>(r)));
+        const int tok = token0 + qi * tile_tokens + r_tok;                 // token inside the sequence
+        const int head = w.head * a.plan.group + r - r_tok * a.plan.group;  // query head
+        const bool mine = r_tok < tile_tokens && tok < w.n;                // (rows left over are walked too; nobody reads them)
+        const long long qpos = static_cast<long long>(p_first) + tok;
+        const int t_lo = qi == 0 ? range[0].lo : range[NQ - 1].lo;
+        const int n_tiles = (qi == 0 ? range[0].hi : range[NQ - 1].hi) - t_lo;
+        const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t tmem_s = tmem_base + qi * kTile;          // S, 128 fp32 columns; P (16-bit, two per column) over the first half
+        const uint32_t tmem_o = tmem_base + C::kTmemO + qi * D;  // O, D fp32 columns
+        const uint32_t my_s_full = bar_s_full + 8 * qi, my_o_full = bar_o_full + 8 * qi;
+        float m_ref = -INFINITY;  // running max in log2 units (scaled, biased)
+        float l_sum = 0.0f;
+        float slope2 = 0.0f;
+        if constexpr (kAlibi) slope2 = mine ? a.alibi_slopes[head] * kLog2e : 0.0f;
+        const float scale2 = a.scale_log2;
+
+        for (int j = 0; j < n_tiles; ++j) {
+            const int cb = t_lo + n_tiles - 1 - j;  // from the last KV tile of this query tile to the first
+            const long long kbase = static_cast<long long>(cb) * kTile;
+            // columns this row may attend to inside the tile: [c_lo, c_hi] (worked out before S arrives)
+            int c_lo = 0, c_hi = kTile - 1;
+            if (mine) {
+                c_hi = min(c_hi, w.keys - 1 - cb * kTile);
+                if (a.plan.is_causal) c_hi = static_cast<int>(min(static_cast<long long>(c_hi), qpos - kbase));
+                if (a.plan.window_right >= 0) c_hi = static_cast<int>(min(static_cast<long long>(c_hi), qpos + a.plan.window_right - kbase));
+                if (a.plan.window_left >= 0) c_lo = static_cast<int>(max(0LL, min(qpos - a.plan.window_left - kbase, 128LL)));
+            }
+            const bool tile_masked = __any_sync(0xffffffffu, c_lo > 0 || c_hi < kTile - 1);
+            if (fail != 0 || !mbar_wait_warp(my_s_full, j & 1, abort_flag)) {
+                // a wait gave up: keep the barrier protocol alive (the MMA warp counts on two arrivals per tile) and do nothing else
+                fail = 8;
+                named_arrive(1 + 2 * qi);
+                named_arrive(2 + 2 * qi);
+                continue;
+            }
+            tc_fence_after_sync();
+
+            float s[128];
+            {
+                uint32_t tmp[4][32];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld32(tmem_s + lane_base + c * 32, tmp[c]);
+                tmem_wait_ld();
+#pragma unroll
+                for (int c = 0; c < 128; ++c) s[c] = __uint_as_float(tmp[c / 32][c % 32]);
+            }
+            if (tile_masked) {
+                // (two passes: a causal diagonal, the common case, needs only the upper bound)
+                if (__any_sync(0xffffffffu, c_hi < kTile - 1)) {
+#pragma unroll
+                    for (int c = 0; c < 128; ++c)
+                        if (c > c_hi) s[c] = -INFINITY;
+                }
+                if (__any_sync(0xffffffffu, c_lo > 0)) {
+#pragma unroll
+                    for (int c = 0; c < 128; ++c)
+                        if (c < c_lo) s[c] = -INFINITY;
+                }
+            }
+            if constexpr (kAlibi) {
+                const float dist0 = static_cast<float>(qpos - kbase);
+#pragma unroll
+                for (int c = 0; c < 128; ++c) s[c] = fmaf(-slope2, fabsf(dist0 - static_cast<float>(c)), s[c] * scale2);
+            }
+            // tile max in log2 units; without ALiBi it is taken over the raw scores and the scale folded into the exponent's FMA
+            float m_tile;
+            {
+                float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                for (int c = 4; c < 128; c += 8) {
+                    mx[0] = max3(mx[0], s[c], s[c + 1]);
+                    mx[1] = max3(mx[1], s[c + 2], s[c + 3]);
+                    if (c + 4 < 128) {
+                        mx[2] = max3(mx[2], s[c + 4], s[c + 5]);
+                        mx[3] = max3(mx[3], s[c + 6], s[c + 7]);
+                    }
+                }
+                m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                if constexpr (!kAlibi) m_tile *= scale2;
+            }
+            // lazy rescale: keep the old reference max unless the new one is much larger
+            float m_new = m_ref, factor = 1.0f;
+            if (m_tile > m_ref + kRescaleThreshold || m_ref == -INFINITY) {
+                m_new = fmaxf(m_ref, m_tile);
+                factor = (m_ref == -INFINITY) ? 0.0f : fast_exp2(m_ref - m_new);
+            }
+            const bool rescale = (j > 0) && (m_new != m_ref);
+            if (__any_sync(0xffffffffu, rescale)) {
+                // P V of the previous tile has completed (its commit precedes s_full), so O is stable.  A row that has seen no key yet
+                // starts from zero, whatever the values of keys that it does not see have left.
+                const float f = rescale ? factor : 1.0f;
+                const uint32_t seen = rescale && m_ref == -INFINITY ? 0u : 0xffffffffu;
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) {
+                    uint32_t orow[32];
+                    tmem_ld32(tmem_o + lane_base + c * 32, orow);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) orow[i] = __float_as_uint(__uint_as_float(orow[i] & seen) * f);
+                    tmem_st32(tmem_o + lane_base + c * 32, orow);
+                }
+            }
+            l_sum *= (m_new != m_ref) ? factor : 1.0f;
+            m_ref = m_new;
+            const float neg_m = (m_ref == -INFINITY) ? 0.0f : -m_ref;
+
+            // P = exp2(s * scale - m), rounded to the inputs' type for the tensor core; its sum is not
+            float2 acc[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
+            const float2 neg_m2 = make_float2(neg_m, neg_m);
+            const float2 scale22 = kAlibi ? make_float2(1.0f, 1.0f) : make_float2(scale2, scale2);
+            auto exp_tile = [&](auto guard_tag) {
+                constexpr bool kGuard = decltype(guard_tag)::value;  // the tile has masked (-inf) scores, for which the polynomial gives 2^-126
+                constexpr uint32_t kPolyMask = poly_mask(D, kAlibi);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {  // quarters of 32 columns
+                    uint32_t pr[16];
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const int col = c * 32 + g * 8 + q * 2;
+                            float2 x = make_float2(s[col], s[col + 1]);
+                            x = __ffma2_rn(x, scale22, neg_m2);
+                            float2 p;
+                            if ((kPolyMask >> ((g & 1) * 4 + q)) & 1u) {
+                                p = poly_exp2_pair(x);
+                                if constexpr (kGuard) {
+                                    if (s[col] == -INFINITY) p.x = 0.0f;
+                                    if (s[col + 1] == -INFINITY) p.y = 0.0f;
+                                }
+                            } else {
+                                p.x = fast_exp2(x.x);
+                                p.y = fast_exp2(x.y);
+                            }
+                            acc[q] = __fadd2_rn(acc[q], p);
+                            pr[g * 4 + q] = pack2<kBf16>(p.x, p.y);
+                        }
+                    }
+                    tmem_st16(tmem_s + lane_base + c * 16, pr);
+                    if (c == (kSplitSteps * 16) / 32 - 1) {
+                        // the first kSplitSteps*16 columns are stored: let the MMA warp start P V on them
+                        tmem_wait_st();
+                        tc_fence_before_sync();
+                        named_arrive(1 + 2 * qi);
+                    }
+                }
+            };
+            if (tile_masked) exp_tile(std::true_type{});
+            else exp_tile(std::false_type{});
+            l_sum += (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y) + (acc[2].x + acc[2].y) + (acc[3].x + acc[3].y);
+            tmem_wait_st();
+            tc_fence_before_sync();
+            named_arrive(2 + 2 * qi);
+        }
+
+        // ---- epilogue: rows of any place, sixteen at a time through this warp's part of the query tile's Q buffer --------------------
+        bool have_o = false;
+        if (n_tiles > 0 && fail == 0) {
+            if (mbar_wait_warp(my_o_full, 0, abort_flag)) { tc_fence_after_sync(); have_o = true; }
+            else fail = 9;
+        }
+        if (!have_o && n_union > 0) (void)mbar_wait_warp(bar_q_full, 0, abort_flag);  // (Q has landed where the rows are staged)
+        const bool gave_up = *abort_flag != 0;
+        if (gave_up) {  // (copies in flight land first)
+            const long long t0 = clock64();
+            while (clock64() - t0 < 200000) { }
+        }
+        // A wait gave up, or a visible page was not there: none of the rows may pass for a softmax.
+        if (gave_up || *bad_page != 0) l_sum = __int_as_float(0x7fc00000);
+        const bool split = w.parts > 1;
+        const long long part_row0 = static_cast<long long>(w.slot + w.part) * a.plan.rows + qi * tile_rows;
+        const float inv = split ? 1.0f : l_sum == 0.0f ? 0.0f : 1.0f / l_sum;  // (NaN stays)
+        // (a row without keys is 0, whatever the values of keys that it does not see have left)
+        auto scaled = [&](uint32_t x) { return l_sum == 0.0f ? 0u : __float_as_uint(__uint_as_float(x) * inv); };
+        if (mine) {
+            if (split) a.ml_partial[part_row0 + r] = make_float2(m_ref, l_sum);
+            else if (a.lse != nullptr)
+                a.lse[static_cast<long long>(w.first + tok) * a.heads + head] = l_sum == 0.0f ? -INFINITY : fmaf(m_ref, kLn2, logf(l_sum));
+        }
+        const uint32_t rows16 = sQ + qi * C::kTileBytes + (warp & 3) * (32 * D * 2);
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+            const int first = (warp & 3) * 32 + h * 16;  // row of the tile
+            const int n_rows = min(16, min(tile_rows, (w.n - token0 - qi * tile_tokens) * a.plan.group) - first);
+            if (n_rows <= 0) break;
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+                uint32_t orow[32];
+                if (have_o) {
+                    tmem_ld32(tmem_o + lane_base + c * 32, orow);
+                    tmem_wait_ld();
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) orow[i] = 0u;
+                }
+                if ((lane >> 4) == h) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        const uint32_t chunk = static_cast<uint32_t>((c * 32 + i) >> 2) ^ static_cast<uint32_t>(lane & 7);
+                        st_shared_v4(rows16 + (lane & 15) * (D * 4) + chunk * 16, scaled(orow[i]), scaled(orow[i + 1]), scaled(orow[i + 2]), scaled(orow[i + 3]));
+                    }
+                }
+                __syncwarp();
+            }
+            constexpr int kLanes = D / 4, kPerWarp = 32 / kLanes;
+            const int chunk = lane % kLanes;
+#pragma unroll 4
+            for (int k = lane / kLanes; k < 16; k += kPerWarp) {
+                if (k >= n_rows || chunk * 4 >= a.head_dim) continue;
+                const float4 o = ld_shared_f32x4(rows16 + k * (D * 4) + static_cast<uint32_t>(chunk ^ (k & 7)) * 16);
+                if (split) {
+                    *reinterpret_cast<float4*>(a.o_partial + (part_row0 + first + k) * D + chunk * 4) = o;
+                    continue;
+                }
+                const int k_tok = static_cast<int>(fast_div(a.div_group, static_cast<uint32_t>(first + k)));
+                const long long at = (w.first + token0 + qi * tile_tokens + k_tok) * a.o_stride[0] +
+                                     (w.head * a.plan.group + first + k - k_tok * a.plan.group) * a.o_stride[1] + chunk * 4;
+                if (a.o_is_fp32) *reinterpret_cast<float4*>(static_cast<float*>(a.o) + at) = o;
+                else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + at) = make_uint2(pack2<kBf16>(o.x, o.y), pack2<kBf16>(o.z, o.w));
+            }
+            __syncwarp();
+        }
+    }
+
+    if (fail != 0) {
+        *abort_flag = 1;
+        if (lane == 0 && a.status != nullptr) atomicExch(a.status, 310 + fail);
+        const long long t0 = clock64();
+        while (clock64() - t0 < 200000) { }
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == C::kMmaWarp && n_union > 0) {
+        __syncwarp();
+        tc_fence_after_sync();
+        tmem_dealloc(tmem_base, C::kTmemCols);
+    }
+}
+
+}  // namespace
+
+template <>
+cudaError_t launch_paged_tiled<FA_PAGED_D, FA_PAGED_NQ>(const PagedArgs& a, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, bool bf16,
+                                                        unsigned grid, cudaStream_t stream) {
+    using C = TCfg<FA_PAGED_D, FA_PAGED_NQ>;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(C::kThreads);
+    cfg.dynamicSmemBytes = C::kSmemBytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    static std::atomic<bool> configured[4][64];
+    auto run = [&](auto kern, std::atomic<bool>* done) -> cudaError_t {
+        if (dev < 0 || dev >= 64 || !done[dev].load(std::memory_order_acquire)) {
+            const cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+            if (err != cudaSuccess) return err;
+            if (dev >= 0 && dev < 64) done[dev].store(true, std::memory_order_release);
+        }
+        return cudaLaunchKernelEx(&cfg, kern, tq, tk, tv, a);
+    };
+    if (a.alibi_slopes != nullptr)
+        return bf16 ? run(paged_tiled_kernel<FA_PAGED_D, FA_PAGED_NQ, true, true>, configured[0])
+                    : run(paged_tiled_kernel<FA_PAGED_D, FA_PAGED_NQ, false, true>, configured[1]);
+    return bf16 ? run(paged_tiled_kernel<FA_PAGED_D, FA_PAGED_NQ, true, false>, configured[2])
+                : run(paged_tiled_kernel<FA_PAGED_D, FA_PAGED_NQ, false, false>, configured[3]);
+}
+
+}  // namespace fa

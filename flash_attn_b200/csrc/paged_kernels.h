@@ -17,6 +17,7 @@ struct PagedArgs {
     long long table_stride;
     int table_width, num_pages, page_shift;
     int heads, head_dim;
+    int tile_tokens;          // tokens of a query tile of 128 rows: 128 / group
     long long q_stride[2], o_stride[2];  // elements from one token and head to the next
     float scale_log2;
     const float* alibi_slopes;
@@ -29,6 +30,14 @@ struct PagedArgs {
 // columns: rows of a block, 1, 4, 8 or 16.
 cudaError_t launch_paged_decode(const PagedArgs& a, const CUtensorMap& tk, const CUtensorMap& tv, int columns, bool bf16, unsigned grid,
                                 cudaStream_t stream);
+// D = 64 or 128 (head_dim rounded up), NQ query tiles a block.
+template <int D, int NQ>
+cudaError_t launch_paged_tiled(const PagedArgs& a, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, bool bf16, unsigned grid,
+                               cudaStream_t stream);
+template <> cudaError_t launch_paged_tiled<64, 1>(const PagedArgs&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, bool, unsigned, cudaStream_t);
+template <> cudaError_t launch_paged_tiled<64, 2>(const PagedArgs&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, bool, unsigned, cudaStream_t);
+template <> cudaError_t launch_paged_tiled<128, 1>(const PagedArgs&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, bool, unsigned, cudaStream_t);
+template <> cudaError_t launch_paged_tiled<128, 2>(const PagedArgs&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, bool, unsigned, cudaStream_t);
 // The split items' rows from their parts.
 cudaError_t launch_paged_combine(const PagedArgs& a, bool bf16, unsigned items, cudaStream_t stream);
 

@@ -210,6 +210,7 @@ __device__ __forceinline__ bool find_work(const PagedPlan& p, PlanScratch<kThrea
             const int per_part = mine.x;
             const int outer = at / per_part;
             w.blk = at - outer * per_part;
+            if (p.is_causal) w.blk = per_part - 1 - w.blk;  // (the longest first)
             w.head = outer / item_parts;
             w.part = outer - w.head * item_parts;
             w.slot = before.z + (w.head * mine.x + w.blk) * parts;
