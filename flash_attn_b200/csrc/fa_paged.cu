@@ -1,5 +1,4 @@
-// Attention of new tokens over a paged K/V cache: the C entry point, its checks and tensor maps, and the kernel that puts the parts of
-// split rows together.
+// Attention of new tokens over a paged K/V cache: the C entry point, its checks, the launch and its tensor maps.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -16,80 +15,9 @@ namespace fa {
 
 namespace {
 
-// A part is not worth starting for fewer tiles than this, and shares above kLongShare are cut into waves.
-constexpr int kMinShare = 4, kLongShare = 24;
-constexpr int kCThreads = 128;
-constexpr int kCRows = 16;  // rows of a CTA of the combine kernel
-
-// One warp per row: O = sum_j 2^(m_j - m) O_j / l, l = sum_j 2^(m_j - m) l_j over the row's parts.  A CTA works the launch's plan out as
-// the kernel before it did, to find its item; it is resident and waiting when that kernel ends.
-template <int D, bool kBf16>
-__global__ void __launch_bounds__(kCThreads) paged_combine_kernel(const __grid_constant__ PagedArgs a) {
-    __shared__ PlanScratch<kCThreads> sm;
-    grid_dep_launch_dependents();
-    grid_dep_wait();
-    PagedWork w;
-    if (!find_work<kCThreads>(a.plan, sm, static_cast<int>(blockIdx.x), true, &w) || w.parts == 1) return;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int row0 = w.blk * a.plan.rows;
-    const int n_rows = min(min(a.plan.rows, w.n * a.plan.group - row0), static_cast<int>(blockIdx.y + 1) * kCRows);
-    const bool mine = lane * 4 < D;
-    for (int n = blockIdx.y * kCRows + warp; n < n_rows; n += kCThreads / 32) {
-        const long long at0 = static_cast<long long>(w.slot) * a.plan.rows + n;  // part j's: + j * plan.rows
-        float m = -INFINITY, l = 0.0f;
-        for (int j = lane; j < w.parts; j += 32) m = fmaxf(m, a.ml_partial[at0 + static_cast<long long>(j) * a.plan.rows].x);
-#pragma unroll
-        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const float base = m == -INFINITY ? 0.0f : m;
-        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int j0 = 0; j0 < w.parts; j0 += 32) {
-            float wt = 0.0f;
-            if (j0 + lane < w.parts) {
-                const float2 ml = a.ml_partial[at0 + static_cast<long long>(j0 + lane) * a.plan.rows];
-                wt = exp2f(ml.x - base);
-                l += ml.x == -INFINITY ? ml.y : wt * ml.y;  // (no key: l = 0; nothing but NaN: NaN)
-            }
-            const int n_parts = min(32, w.parts - j0);
-            for (int j = 0; j < n_parts; j += 8) {
-                float4 v[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (mine && j + i < n_parts)
-                        v[i] = *reinterpret_cast<const float4*>(a.o_partial + (at0 + static_cast<long long>(j0 + j + i) * a.plan.rows) * D + lane * 4);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float x = __shfl_sync(0xffffffffu, wt, (j + i) & 31);
-                    if (mine && j + i < n_parts && x != 0.0f) {
-                        acc.x = fmaf(x, v[i].x, acc.x);
-                        acc.y = fmaf(x, v[i].y, acc.y);
-                        acc.z = fmaf(x, v[i].z, acc.z);
-                        acc.w = fmaf(x, v[i].w, acc.w);
-                    }
-                }
-            }
-        }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // (NaN stays)
-        const int tok = static_cast<int>(fast_div(a.div_group, static_cast<uint32_t>(row0 + n)));
-        const int head = w.head * a.plan.group + row0 + n - tok * a.plan.group;
-        const long long token = w.first + tok;
-        if (lane * 4 < a.head_dim) {
-            const long long at = token * a.o_stride[0] + head * a.o_stride[1] + lane * 4;
-            const float4 o = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-            if (a.o_is_fp32) {
-                *reinterpret_cast<float4*>(static_cast<float*>(a.o) + at) = o;
-            } else if (kBf16) {
-                const __nv_bfloat162 x = __floats2bfloat162_rn(o.x, o.y), y = __floats2bfloat162_rn(o.z, o.w);
-                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + at) = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
-            } else {
-                const __half2 x = __floats2half2_rn(o.x, o.y), y = __floats2half2_rn(o.z, o.w);
-                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + at) = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
-            }
-        }
-        if (lane == 0 && a.lse != nullptr) a.lse[token * a.heads + head] = l == 0.0f ? -INFINITY : fmaf(m, 0.6931471805599453f, logf(l));
-    }
-}
+// A part is not worth starting for fewer tiles than kMinShare; launches of more than one wave are cut into kPagedWaves of parts, which
+// are no shorter than kLongShare.
+constexpr int kMinShare = 4, kLongShare = 24, kPagedWaves = 3;
 
 int check_fwd(const fa_paged_fwd_params* p) {
     if (!p || !p->q || !p->o) return FA_ERR_INVALID_ARG;
@@ -124,8 +52,8 @@ struct PagedLaunch {
     int slots;                 // CTAs that run at once
     int wide;                  // columns of a partial row: head_dim rounded up
     long long items;           // at most so many blocks of rows there are, over all K/V heads
-    long long grid, split_items, partials;
-    size_t o_bytes, bytes;     // workspace: partial rows, and all
+    long long grid, partials;
+    size_t o_bytes, ml_bytes, bytes;  // workspace: partial rows, their maxima and sums, and all
 };
 
 PagedLaunch plan_launch(const fa_paged_fwd_params* p, int sms) {
@@ -145,84 +73,94 @@ PagedLaunch plan_launch(const fa_paged_fwd_params* p, int sms) {
     const long long tiles = (static_cast<long long>(c.table_width) * c.page_size + kTile - 1) / kTile;
     const long long parts = (tiles + kMinShare - 1) / kMinShare;  // of one item
     if (parts > 1) {
-        l.partials = std::min(most_partials(static_cast<int>(slots)), l.items * parts);
-        l.split_items = std::min(l.items, kPagedWaves * slots);
+        // (items longer than the share are cut into less than twice what the shares are)
+        l.partials = std::min(2LL * kPagedWaves * slots, l.items * parts);
     }
     l.grid = l.items + (parts > 1 ? std::min(kPagedWaves * slots, l.items * (parts - 1)) : 0);
     l.o_bytes = (static_cast<size_t>(l.partials) * l.rows * l.wide * sizeof(float) + 255) & ~static_cast<size_t>(255);
-    l.bytes = l.o_bytes + ((static_cast<size_t>(l.partials) * l.rows * sizeof(float2) + 255) & ~static_cast<size_t>(255));
+    l.ml_bytes = (static_cast<size_t>(l.partials) * l.rows * sizeof(float2) + 255) & ~static_cast<size_t>(255);
+    l.bytes = l.o_bytes + l.ml_bytes + ((static_cast<size_t>(l.partials) * 8 + 255) & ~static_cast<size_t>(255));
     return l;
 }
 
-// A 4-D tensor map: dims and strides (elements; of a dimension of one any will do) outermost last.  The last ones are kept per host
-// thread, being a function of these arguments alone.
-int map_of(CUtensorMap* m, int dtype, const void* base, const int64_t (&dims)[4], const int64_t (&strides)[3], const int (&box)[4]) {
+// A tensor map: extents, strides (elements; of a dimension of one any will do) and box, innermost first.  The last ones are kept per
+// host thread, being a function of these arguments alone.
+struct MapShape {
+    const void* base;
+    int dtype, rank;
+    int64_t dims[5], strides[5];  // strides[0]: 1
+    int box[5];
+    bool operator==(const MapShape& o) const {
+        return base == o.base && dtype == o.dtype && rank == o.rank && std::equal(dims, dims + 5, o.dims) && std::equal(strides, strides + 5, o.strides) &&
+               std::equal(box, box + 5, o.box);
+    }
+};
+
+int map_of(CUtensorMap* m, const MapShape& shape) {
     struct Entry {
-        const void* base;
-        int64_t dims[4], strides[3];
-        int box[4], dtype;
-        bool valid;
+        MapShape shape;
         CUtensorMap map;
     };
     constexpr int kEntries = 12;
     thread_local Entry cache[kEntries] = {};
     thread_local int next_victim = 0;
     for (const Entry& e : cache) {
-        if (e.valid && e.base == base && e.dtype == dtype && std::equal(dims, dims + 4, e.dims) && std::equal(strides, strides + 3, e.strides) &&
-            std::equal(box, box + 4, e.box)) {
+        if (e.shape.rank != 0 && e.shape == shape) {
             *m = e.map;
             return FA_OK;
         }
     }
-    cuuint64_t d[4], s[3];
-    cuuint32_t b[4];
-    for (int i = 0; i < 4; ++i) {
-        d[i] = static_cast<cuuint64_t>(dims[i]);
-        b[i] = static_cast<cuuint32_t>(box[i]);
-        if (i > 0) s[i - 1] = dims[i] > 1 ? static_cast<cuuint64_t>(strides[i - 1]) * 2 : 256;
+    cuuint64_t d[5], s[4];
+    cuuint32_t b[5];
+    for (int i = 0; i < shape.rank; ++i) {
+        d[i] = static_cast<cuuint64_t>(shape.dims[i]);
+        b[i] = static_cast<cuuint32_t>(shape.box[i]);
+        if (i > 0) s[i - 1] = shape.dims[i] > 1 ? static_cast<cuuint64_t>(shape.strides[i]) * 2 : 256;
     }
-    const int rc = encode_map(m, dtype, 4, base, d, s, b);
+    const int rc = encode_map(m, shape.dtype, shape.rank, shape.base, d, s, b);
     if (rc != FA_OK) return rc;
     Entry& e = cache[next_victim];
     next_victim = (next_victim + 1) % kEntries;
-    e.base = base;
-    std::copy(dims, dims + 4, e.dims);
-    std::copy(strides, strides + 3, e.strides);
-    std::copy(box, box + 4, e.box);
-    e.dtype = dtype;
+    e.shape = shape;
     e.map = *m;
-    e.valid = true;
     return FA_OK;
 }
 
-// Pages: a box is 64 columns of the tokens of a page (of 128 of them at most) of one head.
-int page_map(CUtensorMap* m, const fa_paged_kv& c, const void* base, const int64_t* stride) {
-    return map_of(m, c.dtype, base, {c.head_dim, c.page_size, c.heads, c.num_pages}, {stride[2], stride[1], stride[0]},
-                  {64, std::min(c.page_size, kTile), 1, 1});
+// The whole-row map of a pool (paged_kernels.h), where its strides allow it.
+bool whole_row_boxes(const fa_paged_kv& c, const void* base, const int64_t* stride, PageBoxes* x, MapShape* shape) {
+    const int64_t eight = 8 * stride[2];
+    if (c.head_dim != 128 || eight <= 0 || eight >= (1LL << 39)) return false;
+    const int64_t page = c.num_pages > 1 ? stride[0] : 0, head = c.heads > 1 ? stride[1] : 0;
+    if (page < 0 || head < 0 || page % eight != 0) return false;
+    const bool apart = head % eight != 0;
+    const int64_t page_step = page / eight, head_step = apart ? 0 : head / eight;
+    const int64_t eights = (c.num_pages - 1) * page_step + (c.heads - 1) * head_step + c.page_size / 8;
+    if (eights >= (1LL << 30)) return false;
+    *x = {static_cast<int>(page_step), static_cast<int>(head_step), apart ? 1 : 0, static_cast<int>(eights)};
+    *shape = {base, c.dtype, 5, {64, 8, 2, eights, apart ? c.heads : 1}, {1, stride[2], 64, eight, head}, {64, 8, 2, std::min(c.page_size, kTile) / 8, 1}};
+    return true;
+}
+
+int page_maps(CUtensorMap* tk, CUtensorMap* tv, const fa_paged_kv& c, PagedArgs* a) {
+    MapShape k, v;
+    a->whole_rows = whole_row_boxes(c, c.k, c.k_stride, &a->k_box, &k) && whole_row_boxes(c, c.v, c.v_stride, &a->v_box, &v);
+    if (!a->whole_rows) {
+        const int box = std::min(c.page_size, kTile);
+        k = {c.k, c.dtype, 4, {c.head_dim, c.page_size, c.heads, c.num_pages}, {1, c.k_stride[2], c.k_stride[1], c.k_stride[0]}, {64, box, 1, 1}};
+        v = {c.v, c.dtype, 4, {c.head_dim, c.page_size, c.heads, c.num_pages}, {1, c.v_stride[2], c.v_stride[1], c.v_stride[0]}, {64, box, 1, 1}};
+    }
+    const int rc = map_of(tk, k);
+    return rc != FA_OK ? rc : map_of(tv, v);
 }
 
 // Q: a box is 64 columns of the rows of a query tile, the heads of one K/V head side by side.
 int query_map(CUtensorMap* m, const fa_paged_fwd_params* p) {
     const int group = p->heads / p->cache.heads;
-    return map_of(m, p->cache.dtype, p->q, {p->cache.head_dim, group, p->cache.heads, p->tokens}, {p->q_stride[1], p->q_stride[1] * group, p->q_stride[0]},
-                  {64, group, 1, kTile / group});
+    return map_of(m, {p->q, p->cache.dtype, 4, {p->cache.head_dim, group, p->cache.heads, p->tokens},
+                      {1, p->q_stride[1], p->q_stride[1] * group, p->q_stride[0]}, {64, group, 1, kTile / group}});
 }
 
 }  // namespace
-
-cudaError_t launch_paged_combine(const PagedArgs& a, bool bf16, unsigned items, cudaStream_t stream) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(items, static_cast<unsigned>((a.plan.rows + kCRows - 1) / kCRows));
-    cfg.blockDim = dim3(kCThreads);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    if (a.head_dim <= 64) return cudaLaunchKernelEx(&cfg, bf16 ? paged_combine_kernel<64, true> : paged_combine_kernel<64, false>, a);
-    return cudaLaunchKernelEx(&cfg, bf16 ? paged_combine_kernel<128, true> : paged_combine_kernel<128, false>, a);
-}
 
 }  // namespace fa
 
@@ -254,11 +192,15 @@ int fa_paged_fwd(const fa_paged_fwd_params* p) {
     a.plan.group = p->heads / c.heads;
     a.plan.rows = l.rows;
     a.plan.is_causal = p->is_causal ? 1 : 0;
-    a.plan.window_left = p->window_left;
-    a.plan.window_right = p->window_right;
+    a.plan.block_tokens = l.rows / a.plan.group + 2;  // (it may begin and end inside a token)
+    a.plan.div_rows = make_fastdiv(static_cast<uint32_t>(l.rows));
+    // (a window of 2^29 or more hides nothing that the cache could hold)
+    a.plan.window_left = p->window_left < kMostKeys / 2 ? p->window_left : -1;
+    a.plan.window_right = p->window_right < kMostKeys / 2 ? p->window_right : -1;
     a.plan.slots = l.slots;
     a.plan.min_share = kMinShare;
     a.plan.long_share = kLongShare;
+    a.plan.waves = kPagedWaves;
     a.plan.partials = static_cast<int>(l.partials);
     a.div_group = make_fastdiv(static_cast<uint32_t>(a.plan.group));
     a.q = p->q;
@@ -281,13 +223,13 @@ int fa_paged_fwd(const fa_paged_fwd_params* p) {
     if (l.bytes > 0) {
         a.o_partial = static_cast<float*>(p->workspace);
         a.ml_partial = reinterpret_cast<float2*>(static_cast<char*>(p->workspace) + l.o_bytes);
+        a.counts = reinterpret_cast<unsigned long long*>(static_cast<char*>(p->workspace) + l.o_bytes + l.ml_bytes);
     }
-    CUtensorMap tk, tv;
-    if ((rc = page_map(&tk, c, c.k, c.k_stride)) != FA_OK) return rc;
-    if ((rc = page_map(&tv, c, c.v, c.v_stride)) != FA_OK) return rc;
     cudaStream_t stream = static_cast<cudaStream_t>(p->stream);
     const bool bf16 = c.dtype == FA_DTYPE_BF16;
     const unsigned grid = static_cast<unsigned>(l.grid);
+    CUtensorMap tk, tv;
+    if ((rc = page_maps(&tk, &tv, c, &a)) != FA_OK) return rc;
     cudaError_t e;
     if (l.columns) {
         e = launch_paged_decode(a, tk, tv, l.columns, bf16, grid, stream);
@@ -297,9 +239,7 @@ int fa_paged_fwd(const fa_paged_fwd_params* p) {
         if (l.wide == 64) e = l.query_tiles == 1 ? launch_paged_tiled<64, 1>(a, tq, tk, tv, bf16, grid, stream) : launch_paged_tiled<64, 2>(a, tq, tk, tv, bf16, grid, stream);
         else e = l.query_tiles == 1 ? launch_paged_tiled<128, 1>(a, tq, tk, tv, bf16, grid, stream) : launch_paged_tiled<128, 2>(a, tq, tk, tv, bf16, grid, stream);
     }
-    if (e != cudaSuccess) return FA_ERR_CUDA;
-    if (l.partials > 0 && launch_paged_combine(a, bf16, static_cast<unsigned>(l.split_items), stream) != cudaSuccess) return FA_ERR_CUDA;
-    return FA_OK;
+    return e == cudaSuccess ? FA_OK : FA_ERR_CUDA;
 }
 
 }  // extern "C"

@@ -17,6 +17,9 @@ bool rows_apart(const int64_t* counts, const int64_t* strides, int n, int64_t co
 // FA_OK, or what of the cache's description the kernels cannot follow.
 int check_cache(const fa_paged_kv& c, int64_t tokens);
 
+// Keys of a sequence; a table has room for no more (check_cache), so that a longer one is named by its missing pages.
+constexpr int kMostKeys = 1 << 30;
+
 // The sequences of a call as the device sees them.
 struct SeqTable {
     const int* seqlens_k;
@@ -34,7 +37,7 @@ __device__ __forceinline__ SeqSpan seq_span(const SeqTable& t, int b) {
     SeqSpan s;
     s.first = t.cu_seqlens_q ? __ldg(t.cu_seqlens_q + b) : b;
     s.end = t.cu_seqlens_q ? __ldg(t.cu_seqlens_q + b + 1) : b + 1;
-    s.keys = max(__ldg(t.seqlens_k + b), 0);
+    s.keys = min(max(__ldg(t.seqlens_k + b), 0), kMostKeys);
     s.first = min(max(s.first, 0), t.tokens);
     s.end = max(min(s.end, t.tokens), s.first);
     return s;

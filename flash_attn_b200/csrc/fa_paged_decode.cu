@@ -5,9 +5,9 @@
 // contiguous K/V, so that the 128 lanes of tensor memory hold KEYS:
 //     S^T[128 keys x 16] = K_tile[128 x d] * Q^T[d x 16],   O^T[d x 16] += V_tile^T[d x 128 keys] * P[128 keys x 16]
 // with the block's rows (a row is a token and a query head; the heads of a K/V head lie side by side) in the first kH columns.
-// A tile of 128 keys is 128 / page_size pages, or a part of one: a lane of the producer warp looks a page up and issues its boxes
-// (64 columns x the tokens of a page, which land as rows of the tile), so that all boxes of a tile leave in one instruction and
-// the lookup's latency hides behind the wait for a free slot.  Pages of which no row sees a key are not looked up.
+// A tile of 128 keys is 128 / page_size pages, or a part of one: a lane of the producer warp looks a page up and issues its box, so
+// that all boxes of a tile leave in one instruction and the lookup's latency hides behind the wait for a free slot.  Pages of which
+// no row sees a key are not looked up.
 //
 // What the pool holds beyond a sequence is not known, and 0 * NaN is NaN: keys that no row sees have P = 0 by their scores, and
 // their rows of a V tile are overwritten with zeros before its MMAs, on the first and last tile of a block.
@@ -18,6 +18,7 @@
 #include <type_traits>
 #include "decode_mma.cuh"
 #include "paged_kernels.h"
+#include "paged_merge.cuh"
 #include "paged_plan.cuh"
 #include "sm100_ptx.cuh"
 
@@ -49,7 +50,7 @@ struct PCfg {
     static constexpr int kSmemReach = kSmemP + (D == 64 ? kTile * 128 : 0);  // V^T is an M = 128 operand: with D = 64 its upper rows read on
     static constexpr int kSmemBytes = (kSmemEnd > kSmemReach ? kSmemEnd : kSmemReach) + 1024;
     static_assert(kSmemBytes <= 115712, "two CTAs per SM");
-    static_assert(sizeof(PlanScratch<kPThreads>) <= kChunk * kOperandBytes, "the plan's scratch lies where P will be");
+    static_assert(sizeof(PlanScratch) <= kChunk * kOperandBytes, "the plan's scratch lies where P will be");
 };
 
 template <bool kBf16, int kH, int D>
@@ -95,7 +96,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
     }
     grid_dep_wait();  // every thread, before its first global access
     PagedWork w;
-    if (!find_work<kPThreads>(a.plan, *reinterpret_cast<PlanScratch<kPThreads>*>(smem_gen + C::kSmemP), static_cast<int>(blockIdx.x), false, &w)) return;
+    if (!find_work<kPThreads>(a.plan, *reinterpret_cast<PlanScratch*>(smem_gen + C::kSmemP), static_cast<int>(blockIdx.x), &w)) return;
 
     // ---- the block's rows and the tiles of this part
     const int row0 = w.blk * kH;                                  // first row: token row0 / group, query head row0 % group of the K/V head
@@ -106,9 +107,10 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
     int vis_lo, vis_hi;
     visible_keys(a.plan, w.keys, p_first + tok_lo, p_first + tok_hi, &vis_lo, &vis_hi);
     const int t_first = vis_lo / kTile, t_all = vis_hi > vis_lo ? (vis_hi + kTile - 1) / kTile - t_first : 0;
-    const int lo = t_first + static_cast<int>(static_cast<long long>(t_all) * w.part / w.parts);
-    const int hi = t_first + static_cast<int>(static_cast<long long>(t_all) * (w.part + 1) / w.parts);
-    const int n_tiles = hi - lo;
+    int lo, hi;
+    part_of(t_all, w.part, w.parts, &lo, &hi);
+    lo += t_first;
+    const int n_tiles = hi + t_first - lo;
     // tiles [full_lo, full_hi) need no mask: every row sees all of their keys
     int full_lo, full_hi;
     {
@@ -125,29 +127,14 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
         tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), kPTmemCols);
         tmem_relinquish();
     }
-    // ---- producer: page `lane / halves` of a tile, columns 64 * (lane % halves)
-    const int page_rows = min(1 << a.page_shift, kTile);   // tokens of a box
-    const int tile_pages = kTile / page_rows;
-    const int my_page = lane / kHalves, my_half = lane % kHalves;
+    // ---- producer
+    const PageLane mine = page_lane<kHalves>(a, lane);
     const int* table = a.page_table + w.b * a.table_stride;
     bool met_bad = false;
-    auto lookup = [&](int tile) -> int {  // the page that this lane loads, -1: none (no row sees a key of it)
-        const int key = tile * kTile + my_page * page_rows;
-        if (my_page >= tile_pages || key >= vis_hi || key + page_rows <= vis_lo) return -1;
-        const int nth = key >> a.page_shift;
-        const int page = nth < a.table_width ? __ldg(table + nth) : -1;
-        if (page >= 0 && page < a.num_pages) return page;
-        met_bad = true;
-        return a.num_pages;  // outside of the tensor map: the box is zeros
-    };
-    auto load = [&](const CUtensorMap* map, int st, int tile, int page) {
-        const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, page >= 0));
+    auto lookup = [&](int tile) { return page_lookup(a, mine, table, tile, vis_lo, vis_hi, &met_bad); };
+    auto load = [&](bool of_k, int st, int tile, int page) {
         if (__any_sync(0xffffffffu, met_bad) && lane == 0) *bad_page = 1;  // (before what the readers' barriers wait for)
-        if (lane == 0) mbar_expect_tx(bar_full + 8 * st, boxes * page_rows * 128);
-        __syncwarp();
-        if (page >= 0)
-            tma_load_4d(sRing + st * kTileBytes + my_half * (kTile * 128) + my_page * (page_rows * 128), map, bar_full + 8 * st, my_half * 64,
-                        (tile * kTile) & ((1 << a.page_shift) - 1), w.head, page);
+        page_load<kHalves>(a, of_k ? a.k_box : a.v_box, mine, of_k ? &tmap_k : &tmap_v, sRing + st * kTileBytes, bar_full + 8 * st, tile, w.head, page);
     };
     int pushed = 0;  // tiles whose loads have been issued (producer warp only)
     if (warp == 4) {
@@ -158,7 +145,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
         for (int i = 0; i < (kStages < kChunkTiles ? kStages : kChunkTiles); ++i) page[i] = i < first ? lookup(lo + i) : -1;
 #pragma unroll
         for (int i = 0; i < (kStages < kChunkTiles ? kStages : kChunkTiles); ++i)
-            if (i < first) load(&tmap_k, i, lo + i, page[i]);
+            if (i < first) load(true, i, lo + i, page[i]);
         pushed = first;
     }
     const long long token0 = w.first;
@@ -188,25 +175,25 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
     if (n_tiles > 0 && warp == 4) {
         // ======================= TMA producer ===================================
         int slot = 0;  // running count of tiles in stream order: K(0), K(1), V(0), K(2), V(1), ... (chunks)
-        auto push = [&](const CUtensorMap* map, int tile) -> bool {
+        auto push = [&](bool of_k, int tile) -> bool {
             if (slot < pushed) { ++slot; return true; }  // issued during set-up
             const int st = slot % kStages;
             const uint32_t ph = (slot / kStages) & 1;
             const int page = lookup(tile);
             if (!mbar_wait_warp_ok(bar_empty + 8 * st, ph ^ 1, abort_flag)) return false;
-            load(map, st, tile, page);
+            load(of_k, st, tile, page);
             ++slot;
             return true;
         };
-        auto push_chunk = [&](const CUtensorMap* map, int c) -> bool {
+        auto push_chunk = [&](bool of_k, int c) -> bool {
             for (int t = 0; t < chunk_tiles(c); ++t)
-                if (!push(map, lo + c * kChunkTiles + t)) return false;
+                if (!push(of_k, lo + c * kChunkTiles + t)) return false;
             return true;
         };
-        bool ok = push_chunk(&tmap_k, 0);
+        bool ok = push_chunk(true, 0);
         for (int c = 0; ok && c < n_chunks; ++c) {
-            if (c + 1 < n_chunks) ok = push_chunk(&tmap_k, c + 1);
-            if (ok) ok = push_chunk(&tmap_v, c);
+            if (c + 1 < n_chunks) ok = push_chunk(true, c + 1);
+            if (ok) ok = push_chunk(false, c);
         }
         if (!ok) fail = 1;
         if (__any_sync(0xffffffffu, met_bad) && lane == 0 && a.status != nullptr) atomicExch(a.status, FA_STATUS_PAGE);
@@ -214,6 +201,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
         // ======================= MMA issuer =====================================
         constexpr uint32_t idesc_qk = make_idesc_swapped(kBf16, false);
         constexpr uint32_t idesc_pv = make_idesc_swapped(kBf16, true);
+        // bytes from eight keys of a tile to the next, and from their first 64 columns to the others
+        const uint32_t eight_bytes = D == 128 && a.whole_rows ? 2048 : 1024, half_bytes = D == 128 && a.whole_rows ? 1024 : kTile * 128;
         int slot = 0;
         auto qk_chunk = [&](int c) -> bool {
             const int buf = c & 1;
@@ -227,9 +216,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
                 if (lane == 0) {
 #pragma unroll
                     for (int ks = 0; ks < D / 16; ++ks) {
-                        const uint32_t off = (ks / 4) * (kTile * 128) + (ks % 4) * 32;
+                        const uint32_t off = (ks / 4) * half_bytes + (ks % 4) * 32;
                         const uint32_t qoff = (ks / 4) * C::kHalfBytes + (ks % 4) * 32;
-                        umma_ss(tmem_base + buf * 64 + t * 16, make_smem_desc(kt + off, 0, 1024), make_smem_desc(sQ + qoff, 0, 1024), idesc_qk,
+                        umma_ss(tmem_base + buf * 64 + t * 16, make_smem_desc(kt + off, 0, eight_bytes), make_smem_desc(sQ + qoff, 0, 1024), idesc_qk,
                                 ks > 0 ? 1u : 0u);
                     }
                     umma_commit(bar_empty + 8 * st);
@@ -250,20 +239,14 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
                 const int key0 = (lo + c * kChunkTiles + t) * kTile;
                 if (key0 < vis_lo || key0 + kTile > vis_hi) {
                     // rows that no query row sees may hold anything
-                    const int head = max(vis_lo - key0, 0), tail = min(max(vis_hi - key0, 0), kTile);
-                    for (int i = lane; i < kTile * kHalves * 8; i += 32) {
-                        const int row = (i >> 3) % kTile;
-                        if (row < head || row >= tail) st_shared_v4(vt + i * 16, 0u, 0u, 0u, 0u);
-                    }
-                    fence_proxy_async_smem();
-                    __syncwarp();
+                    clear_rows<kHalves>(a, vt, max(vis_lo - key0, 0), min(max(vis_hi - key0, 0), kTile));
                 }
                 if (lane == 0) {
 #pragma unroll
                     for (int ks = 0; ks < 8; ++ks) {
-                        // A = V^T: 16 keys (2048 bytes) per step, the two 64-column halves 16 KB apart
+                        // A = V^T: 16 keys a step
                         const uint32_t poff = t * C::kOperandBytes + (ks / 4) * C::kHalfBytes + (ks % 4) * 32;
-                        umma_ss(tmem_o, make_smem_desc(vt + ks * 2048, kTile * 128, 1024), make_smem_desc(sP + poff, 0, 1024), idesc_pv,
+                        umma_ss(tmem_o, make_smem_desc(vt + ks * 2 * eight_bytes, half_bytes, eight_bytes), make_smem_desc(sP + poff, 0, 1024), idesc_pv,
                                 (c > 0 || t > 0 || ks > 0) ? 1u : 0u);
                     }
                     umma_commit(bar_empty + 8 * st);
@@ -461,7 +444,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
             const int tok = __shfl_sync(0xffffffffu, my_tok, n), head = __shfl_sync(0xffffffffu, my_head, n);
             if (n >= nc) continue;
             const float l_sum = (red[8 * kH + n] + red[9 * kH + n]) + (red[10 * kH + n] + red[11 * kH + n]) + spoilt;
-            if (w.parts > 1) {  // un-normalised, for the combine kernel
+            if (w.parts > 1) {  // un-normalised, for the last part to come
                 const long long at = static_cast<long long>(w.slot + w.part) * kH + n;
                 if (r < D) a.o_partial[at * D + r] = __uint_as_float(o_raw[n]);
                 if (r == 0) a.ml_partial[at] = make_float2(m_n, l_sum);
@@ -477,6 +460,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
                     a.lse[(token0 + tok) * a.heads + head] = l_sum == 0.0f ? -INFINITY : fmaf(m_n, kPLn2, logf(l_sum));
             }
         }
+        if (w.parts > 1 && last_to_come<128>(a, w, reinterpret_cast<volatile int*>(smem_gen + C::kSmemMisc + 12)))
+            merge_parts<D, kBf16, 4>(a, w, row0, nc, warp);
     }
 
     if (fail != 0) {

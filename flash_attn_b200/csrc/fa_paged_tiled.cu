@@ -16,6 +16,7 @@
 #include <cuda_fp16.h>
 #include <type_traits>
 #include "paged_kernels.h"
+#include "paged_merge.cuh"
 #include "paged_plan.cuh"
 #include "sm100_ptx.cuh"
 #include "tiled_mma.cuh"
@@ -35,6 +36,44 @@ constexpr float kLn2 = 0.6931471805599453f;
 
 // Column pairs that take the polynomial exp2, a quarter of them (see the tiled kernel for contiguous K/V).
 __host__ __device__ constexpr uint32_t poly_mask(int d, bool alibi) { return alibi ? 0x11u : d == 128 ? 0x88u : 0x81u; }
+
+// The MMAs of one S = Q K^T tile in one asm block, so that the issuing thread does no other work between them (16-byte units: a k-step
+// is 2 inside 64 columns; Q's next 64 columns lie 16 KB further, K's `k_jump` past their last step).
+#define FA_PAGED_QK(qi, ki)                                                                    \
+    "add.u32 qa, qa, " qi ";\n\tadd.u32 kb, kb, " ki ";\n\t"                                     \
+    "mov.b64 da, {qa, %3};\n\tmov.b64 db, {kb, %4};\n\t"                                        \
+    "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p1;\n\t"
+template <int D>
+__device__ __forceinline__ void issue_qk(uint32_t d_tmem, uint32_t q_lo, uint32_t k_lo, uint32_t q_hi, uint32_t k_hi, uint32_t k_jump, uint32_t idesc) {
+#define FA_PAGED_QK_HEAD                                                                       \
+    "{\n\t.reg .pred p0, p1;\n\t.reg .b32 qa, kb;\n\t.reg .b64 da, db;\n\t"                       \
+    "setp.ne.b32 p0, 0, 0;\n\tsetp.eq.b32 p1, 0, 0;\n\tmov.b32 qa, %1;\n\tmov.b32 kb, %2;\n\t"      \
+    "mov.b64 da, {qa, %3};\n\tmov.b64 db, {kb, %4};\n\t"                                        \
+    "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p0;\n\t"
+    if constexpr (D == 128) {
+        asm volatile(FA_PAGED_QK_HEAD FA_PAGED_QK("2", "2") FA_PAGED_QK("2", "2") FA_PAGED_QK("2", "2") FA_PAGED_QK("1018", "%6") FA_PAGED_QK("2", "2")
+                         FA_PAGED_QK("2", "2") FA_PAGED_QK("2", "2") "}"
+                     ::"r"(d_tmem), "r"(q_lo), "r"(k_lo), "r"(q_hi), "r"(k_hi), "r"(idesc), "r"(k_jump)
+                     : "memory");
+    } else {
+        asm volatile(FA_PAGED_QK_HEAD FA_PAGED_QK("2", "2") FA_PAGED_QK("2", "2") FA_PAGED_QK("2", "2") "}"
+                     ::"r"(d_tmem), "r"(q_lo), "r"(k_lo), "r"(q_hi), "r"(k_hi), "r"(idesc)
+                     : "memory");
+    }
+}
+// Four MMAs of O += P V, from k-step kFrom on: P advances 8 columns of tensor memory a step, V `v_step`.
+#define FA_PAGED_PV                                                                            \
+    "add.u32 pa, pa, 8;\n\tadd.u32 vb, vb, %6;\n\tmov.b64 db, {vb, %3};\n\t"                       \
+    "tcgen05.mma.cta_group::1.kind::f16 [%0], [pa], db, %4, p1;\n\t"
+template <int kFrom>
+__device__ __forceinline__ void issue_pv(uint32_t d_tmem, uint32_t p_tmem, uint32_t v_lo, uint32_t v_hi, uint32_t v_step, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p0, p1;\n\t.reg .b32 pa, vb;\n\t.reg .b64 db;\n\t"
+        "setp.ne.b32 p0, %5, 0;\n\tsetp.eq.b32 p1, 0, 0;\n\tmov.b32 pa, %1;\n\tmov.b32 vb, %2;\n\tmov.b64 db, {vb, %3};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [pa], db, %4, p0;\n\t" FA_PAGED_PV FA_PAGED_PV FA_PAGED_PV "}"
+        ::"r"(d_tmem), "r"(p_tmem + kFrom * 8), "r"(v_lo + kFrom * v_step), "r"(v_hi), "r"(idesc), "r"(accumulate), "r"(v_step)
+        : "memory");
+}
 
 template <int D, int NQ>
 struct TCfg {
@@ -58,7 +97,7 @@ struct TCfg {
     static constexpr int kNumBars = 1 + 2 * NQ + 4 * kStages;
     static constexpr int kSmemMisc = kSmemBar + 8 * kNumBars;  // tensor-memory address, abort flag, bad page
     static constexpr int kSmemPlan = (kSmemMisc + 16 + 15) / 16 * 16;
-    static constexpr int kSmemBytes = kSmemPlan + static_cast<int>(sizeof(PlanScratch<kThreads>)) + 1024;  // + alignment slack
+    static constexpr int kSmemBytes = kSmemPlan + static_cast<int>(sizeof(PlanScratch)) + 1024;  // + alignment slack
     static_assert(kSmemBytes <= (NQ == 2 ? 232448 : 115712), "one or two CTAs per SM");
 };
 
@@ -98,7 +137,7 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     }
     grid_dep_wait();  // every thread, before its first global access
     PagedWork w;
-    if (!find_work<C::kThreads>(a.plan, *reinterpret_cast<PlanScratch<C::kThreads>*>(smem_gen + C::kSmemPlan), static_cast<int>(blockIdx.x), false, &w))
+    if (!find_work<C::kThreads>(a.plan, *reinterpret_cast<PlanScratch*>(smem_gen + C::kSmemPlan), static_cast<int>(blockIdx.x), &w))
         return;
 
     // ---- the block's query tiles, and the tiles of keys of this part
@@ -122,8 +161,10 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     }
     const int n_all = hi > lo ? hi - lo : 0, lo_all = hi > lo ? lo : 0;
     if (w.parts > 1) {
-        const int p_lo = lo_all + static_cast<int>(static_cast<long long>(n_all) * w.part / w.parts);
-        const int p_hi = lo_all + static_cast<int>(static_cast<long long>(n_all) * (w.part + 1) / w.parts);
+        int p_lo, p_hi;
+        part_of(n_all, w.part, w.parts, &p_lo, &p_hi);
+        p_lo += lo_all;
+        p_hi += lo_all;
         lo = 0x7fffffff;
         hi = 0;
 #pragma unroll
@@ -139,28 +180,13 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     const int n_union = hi > lo ? hi - lo : 0;  // KV tiles of this CTA: [lo, hi)
 
     // ---- set-up: loads of Q and the first K/V tiles, tensor memory
-    const int page_rows = min(1 << a.page_shift, kTile);  // tokens of a box
-    const int tile_pages = kTile / page_rows;
-    const int my_page = lane / C::kBoxes, my_box = lane % C::kBoxes;
+    const PageLane page_box = page_lane<C::kBoxes>(a, lane);
     const int* table = a.page_table + w.b * a.table_stride;
     bool met_bad = false;
-    auto lookup = [&](int tile) -> int {  // the page that this lane loads, -1: none (no row of the block sees a key of it)
-        const int key = tile * kTile + my_page * page_rows;
-        if (my_page >= tile_pages || key >= vis_hi || key + page_rows <= vis_lo) return -1;
-        const int nth = key >> a.page_shift;
-        const int page = nth < a.table_width ? __ldg(table + nth) : -1;
-        if (page >= 0 && page < a.num_pages) return page;
-        met_bad = true;
-        return a.num_pages;  // outside of the tensor map: the box is zeros
-    };
-    auto load = [&](const CUtensorMap* map, uint32_t dst, uint32_t bar, int tile, int page) {
-        const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, page >= 0));
+    auto lookup = [&](int tile) { return page_lookup(a, page_box, table, tile, vis_lo, vis_hi, &met_bad); };
+    auto load = [&](bool of_k, uint32_t dst, uint32_t bar, int tile, int page) {
         if (__any_sync(0xffffffffu, met_bad) && lane == 0) *bad_page = 1;  // (before what the readers' barriers wait for)
-        if (lane == 0) mbar_expect_tx(bar, boxes * page_rows * 128);
-        __syncwarp();
-        if (page >= 0)
-            tma_load_4d(dst + my_box * (kTile * 128) + my_page * (page_rows * 128), map, bar, my_box * 64,
-                        (tile * kTile) & ((1 << a.page_shift) - 1), w.head, page);
+        page_load<C::kBoxes>(a, of_k ? a.k_box : a.v_box, page_box, of_k ? &tmap_k : &tmap_v, dst, bar, tile, w.head, page);
     };
     int prefilled = 0;
     if (warp == C::kProducerWarp && n_union > 0) {
@@ -180,8 +206,8 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
 #pragma unroll
         for (int t = 0; t < C::kStages; ++t) {  // KV tiles are walked from the last to the first
             if (t >= prefilled) break;
-            load(&tmap_k, sK + t * C::kTileBytes, bar_k_full + 8 * t, hi - 1 - t, page[t]);
-            load(&tmap_v, sV + t * C::kTileBytes, bar_v_full + 8 * t, hi - 1 - t, page[t]);
+            load(true, sK + t * C::kTileBytes, bar_k_full + 8 * t, hi - 1 - t, page[t]);
+            load(false, sV + t * C::kTileBytes, bar_v_full + 8 * t, hi - 1 - t, page[t]);
         }
     }
     if (warp == C::kMmaWarp && n_union > 0) {
@@ -203,9 +229,9 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                 const uint32_t ph = (t / C::kStages) & 1;
                 const int tile = hi - 1 - t, page = lookup(tile);
                 if (!mbar_wait_warp(bar_k_empty + 8 * st, ph ^ 1, abort_flag)) { fail = 1; break; }
-                load(&tmap_k, sK + st * C::kTileBytes, bar_k_full + 8 * st, tile, page);
+                load(true, sK + st * C::kTileBytes, bar_k_full + 8 * st, tile, page);
                 if (!mbar_wait_warp(bar_v_empty + 8 * st, ph ^ 1, abort_flag)) { fail = 2; break; }
-                load(&tmap_v, sV + st * C::kTileBytes, bar_v_full + 8 * st, tile, page);
+                load(false, sV + st * C::kTileBytes, bar_v_full + 8 * st, tile, page);
             }
             if (__any_sync(0xffffffffu, met_bad) && lane == 0 && a.status != nullptr) atomicExch(a.status, FA_STATUS_PAGE);
         } else if (n_union > 0 && warp == C::kMmaWarp) {
@@ -213,12 +239,14 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             const bool leader = elect_one();
             constexpr uint32_t idesc_qk = make_idesc_f16(kTile, kTile, kBf16, false);
             constexpr uint32_t idesc_pv = make_idesc_f16(kTile, D, kBf16, true);
-            const uint64_t dqk = make_smem_desc(0, 0, 1024);
-            const uint64_t dvv = make_smem_desc(0, kTile * 128, 1024);
-            const uint32_t desc_hi = static_cast<uint32_t>(dqk >> 32);
-            const uint32_t q_lo = static_cast<uint32_t>(dqk) | (sQ >> 4), k_lo = static_cast<uint32_t>(dqk) | (sK >> 4), v_lo = static_cast<uint32_t>(dvv) | (sV >> 4);
-            auto issue_qk = [&](int i, int st) {
-                issue_qk_block<D>(tmem_base + i * kTile, q_lo + ((i * C::kTileBytes) >> 4), k_lo + ((st * C::kTileBytes) >> 4), desc_hi, idesc_qk);
+            // bytes from eight keys of a tile to the next, and from their first 64 columns to the others
+            const uint32_t eight_bytes = D == 128 && a.whole_rows ? 2048 : 1024, half_bytes = D == 128 && a.whole_rows ? 1024 : kTile * 128;
+            const uint64_t dq = make_smem_desc(0, 0, 1024), dk = make_smem_desc(0, 0, eight_bytes), dv = make_smem_desc(0, half_bytes, eight_bytes);
+            const uint32_t q_hi = static_cast<uint32_t>(dq >> 32), kv_hi = static_cast<uint32_t>(dk >> 32);
+            const uint32_t q_lo = static_cast<uint32_t>(dq) | (sQ >> 4), k_lo = static_cast<uint32_t>(dk) | (sK >> 4), v_lo = static_cast<uint32_t>(dv) | (sV >> 4);
+            const uint32_t k_jump = half_bytes / 16 - 6, v_step = eight_bytes / 8;
+            auto issue_s = [&](int i, int st) {
+                issue_qk<D>(tmem_base + i * kTile, q_lo + ((i * C::kTileBytes) >> 4), k_lo + ((st * C::kTileBytes) >> 4), q_hi, kv_hi, k_jump, idesc_qk);
             };
             auto active = [&](int i, int tile) { return tile >= range[i].lo && tile < range[i].hi; };
             do {
@@ -229,7 +257,7 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
 #pragma unroll
                     for (int i = 0; i < NQ; ++i) {
                         if (active(i, hi - 1)) {
-                            issue_qk(i, 0);
+                            issue_s(i, 0);
                             umma_commit(bar_s_full + 8 * i);
                         }
                     }
@@ -245,14 +273,7 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                     if (!mbar_wait_warp(bar_v_full + 8 * st, ph, abort_flag)) { fail = 6; break; }
                     if (tile * kTile < vis_lo || tile * kTile + kTile > vis_hi) {
                         // keys that no row of the block sees: their rows of V may hold anything
-                        const int head = max(vis_lo - tile * kTile, 0), tail = min(vis_hi - tile * kTile, kTile);
-                        const uint32_t v = sV + st * C::kTileBytes;
-                        for (int j = lane; j < kTile * C::kBoxes * 8; j += 32) {
-                            const int row = (j >> 3) % kTile;
-                            if (row < head || row >= tail) st_shared_v4(v + j * 16, 0u, 0u, 0u, 0u);
-                        }
-                        fence_proxy_async_smem();
-                        __syncwarp();
+                        clear_rows<C::kBoxes>(a, sV + st * C::kTileBytes, max(vis_lo - tile * kTile, 0), min(vis_hi - tile * kTile, kTile));
                     }
                     if (more) {
                         if (!mbar_wait_warp(bar_k_full + 8 * st1, ph1, abort_flag)) { fail = 7; break; }
@@ -264,18 +285,18 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                             named_sync(1 + 2 * i);
                             tc_fence_after_sync();
                             if (leader)
-                                issue_pv_first(tmem_base + C::kTmemO + i * D, tmem_base + i * kTile, v_lo + ((st * C::kTileBytes) >> 4), desc_hi, idesc_pv,
+                                issue_pv<0>(tmem_base + C::kTmemO + i * D, tmem_base + i * kTile, v_lo + ((st * C::kTileBytes) >> 4), kv_hi, v_step, idesc_pv,
                                                tile < range[i].hi - 1 ? 1u : 0u);
                             named_sync(2 + 2 * i);
                             tc_fence_after_sync();
                             if (leader) {
-                                issue_pv_rest(tmem_base + C::kTmemO + i * D, tmem_base + i * kTile, v_lo + ((st * C::kTileBytes) >> 4), desc_hi, idesc_pv);
+                                issue_pv<kSplitSteps>(tmem_base + C::kTmemO + i * D, tmem_base + i * kTile, v_lo + ((st * C::kTileBytes) >> 4), kv_hi, v_step, idesc_pv, 1u);
                                 if (tile == range[i].lo) umma_commit(bar_o_full + 8 * i);
                             }
                         }
                         if (more && active(i, tile - 1)) {
                             if (leader) {
-                                issue_qk(i, st1);
+                                issue_s(i, st1);
                                 umma_commit(bar_s_full + 8 * i);
                             }
                         }
@@ -296,7 +317,7 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         const int tok = token0 + qi * tile_tokens + r_tok;                 // token inside the sequence
         const int head = w.head * a.plan.group + r - r_tok * a.plan.group;  // query head
         const bool mine = r_tok < tile_tokens && tok < w.n;                // (rows left over are walked too; nobody reads them)
-        const long long qpos = static_cast<long long>(p_first) + tok;
+        const int qpos = p_first + tok;
         const int t_lo = qi == 0 ? range[0].lo : range[NQ - 1].lo;
         const int n_tiles = (qi == 0 ? range[0].hi : range[NQ - 1].hi) - t_lo;
         const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -311,14 +332,14 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
 
         for (int j = 0; j < n_tiles; ++j) {
             const int cb = t_lo + n_tiles - 1 - j;  // from the last KV tile of this query tile to the first
-            const long long kbase = static_cast<long long>(cb) * kTile;
+            const int kbase = cb * kTile;
             // columns this row may attend to inside the tile: [c_lo, c_hi] (worked out before S arrives)
             int c_lo = 0, c_hi = kTile - 1;
             if (mine) {
                 c_hi = min(c_hi, w.keys - 1 - cb * kTile);
-                if (a.plan.is_causal) c_hi = static_cast<int>(min(static_cast<long long>(c_hi), qpos - kbase));
-                if (a.plan.window_right >= 0) c_hi = static_cast<int>(min(static_cast<long long>(c_hi), qpos + a.plan.window_right - kbase));
-                if (a.plan.window_left >= 0) c_lo = static_cast<int>(max(0LL, min(qpos - a.plan.window_left - kbase, 128LL)));
+                if (a.plan.is_causal) c_hi = min(c_hi, qpos - kbase);
+                if (a.plan.window_right >= 0) c_hi = min(c_hi, qpos + a.plan.window_right - kbase);
+                if (a.plan.window_left >= 0) c_lo = max(0, min(qpos - a.plan.window_left - kbase, kTile));
             }
             const bool tile_masked = __any_sync(0xffffffffu, c_lo > 0 || c_hi < kTile - 1);
             if (fail != 0 || !mbar_wait_warp(my_s_full, j & 1, abort_flag)) {
@@ -515,6 +536,8 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             }
             __syncwarp();
         }
+        if (split && last_to_come<NQ * 128>(a, w, reinterpret_cast<volatile int*>(smem_gen + C::kSmemMisc + 12)))
+            merge_parts<D, kBf16, NQ * 4>(a, w, token0 * a.plan.group, min(a.plan.rows, (w.n - token0) * a.plan.group), warp);
     }
 
     if (fail != 0) {

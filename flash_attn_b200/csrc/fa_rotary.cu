@@ -356,6 +356,7 @@ int check_cache(const fa_paged_kv& c, int64_t tokens) {
         }
         if (!rows_apart(counts, s, 3, c.head_dim)) return FA_ERR_INVALID_ARG;
     }
+    if (static_cast<long long>(c.table_width) * c.page_size >= kMostKeys) return FA_ERR_TOO_LARGE;
     if (tokens > 0x3fffffffLL || c.batch > 0x3fffffff) return FA_ERR_TOO_LARGE;
     if (!c.cu_seqlens_q && tokens < c.batch) return FA_ERR_INVALID_ARG;
     return FA_OK;
