@@ -13,6 +13,7 @@
 #include <cmath>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <type_traits>
 #include "fa_internal.h"
 #include "fa_paged.h"
 #include "sm100_ptx.cuh"
@@ -22,21 +23,57 @@ namespace fa {
 namespace {
 
 constexpr int kRThreads = 256;
+// Blocks an SM: 96 KB of loads in flight.  (bf16 [4, 32, 4096, 128]: with two blocks 44.0 us, three 42.2, four and two heads in flight
+// 43.1; 6.4 TB/s.)
+constexpr int kRBlocks = 3;
 constexpr int kRUnroll = 4;       // heads whose vectors a thread has in flight
 constexpr int kSeqStage = 1024;   // row numbers of sequences that a block keeps in shared memory
 
-__device__ __forceinline__ float widen(float x) { return x; }
-__device__ __forceinline__ float widen(__half x) { return __half2float(x); }
-__device__ __forceinline__ float widen(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <typename T> __device__ __forceinline__ T narrow(float x);
-template <> __device__ __forceinline__ float narrow<float>(float x) { return x; }
-template <> __device__ __forceinline__ __half narrow<__half>(float x) { return __float2half_rn(x); }
-template <> __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
-
-// kVec consecutive elements, loaded and stored as one.
+// kVec consecutive elements, loaded and stored as one and kept as they lie in memory: unpacked, 16-bit elements take a register each.
 template <typename T, int kVec>
-struct alignas(sizeof(T) * kVec) Vec {
-    T e[kVec];
+struct Vec {
+    static constexpr int kBytes = static_cast<int>(sizeof(T)) * kVec, kWords = (kBytes + 3) / 4;
+    uint32_t w[kWords];
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (kBytes == 16) {
+            const uint4 v = *reinterpret_cast<const uint4*>(p);
+            w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+        } else if constexpr (kBytes == 8) {
+            const uint2 v = *reinterpret_cast<const uint2*>(p);
+            w[0] = v.x; w[1] = v.y;
+        } else if constexpr (kBytes == 4) {
+            w[0] = *reinterpret_cast<const uint32_t*>(p);
+        } else {
+            w[0] = *reinterpret_cast<const uint16_t*>(p);
+        }
+    }
+    __device__ __forceinline__ void store(T* p) const {
+        if constexpr (kBytes == 16) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+        else if constexpr (kBytes == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+        else if constexpr (kBytes == 4) *reinterpret_cast<uint32_t*>(p) = w[0];
+        else *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(w[0]);
+    }
+    __device__ __forceinline__ float get(int i) const {
+        if constexpr (std::is_same_v<T, float>) return __uint_as_float(w[i]);
+        else if constexpr (std::is_same_v<T, __nv_bfloat16>) return __uint_as_float((i & 1) ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
+        else return __half2float(__ushort_as_half(static_cast<unsigned short>((i & 1) ? w[i >> 1] >> 16 : w[i >> 1])));
+    }
+    // elements i and i + 1 (i even; of a single element: x)
+    __device__ __forceinline__ void set2(int i, float x, float y) {
+        if constexpr (std::is_same_v<T, float>) {
+            w[i] = __float_as_uint(x);
+            if constexpr (kVec > 1) w[i + 1] = __float_as_uint(y);
+        } else if constexpr (kVec == 1) {
+            if constexpr (std::is_same_v<T, __nv_bfloat16>) w[0] = __bfloat16_as_ushort(__float2bfloat16_rn(x));
+            else w[0] = __half_as_ushort(__float2half_rn(x));
+        } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+            const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+            w[i >> 1] = *reinterpret_cast<const uint32_t*>(&v);
+        } else {
+            const __half2 v = __floats2half2_rn(x, y);
+            w[i >> 1] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+    }
 };
 
 struct Rotation {
@@ -87,17 +124,27 @@ __device__ __forceinline__ void angles(const Rotation& r, int group, long long p
 
 template <typename T, int kVec, bool kInterleaved>
 __device__ __forceinline__ void turn(Vec<T, kVec>& va, Vec<T, kVec>& vb, const float (&cs)[kVec], const float (&sn)[kVec]) {
+    if constexpr (kInterleaved && kVec > 1) {  // pairs 0 .. kVec/2-1 lie in the first vector, the others in the second
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) {
-        if constexpr (kInterleaved && kVec > 1) {  // pairs 0 .. kVec/2-1 lie in the first vector, the others in the second
-            T* p = i < kVec / 2 ? va.e + 2 * i : vb.e + 2 * i - kVec;
-            const float x = widen(p[0]), y = widen(p[1]);
-            p[0] = narrow<T>(fmaf(x, cs[i], -(y * sn[i])));
-            p[1] = narrow<T>(fmaf(y, cs[i], x * sn[i]));
-        } else {
-            const float x = widen(va.e[i]), y = widen(vb.e[i]);
-            va.e[i] = narrow<T>(fmaf(x, cs[i], -(y * sn[i])));
-            vb.e[i] = narrow<T>(fmaf(y, cs[i], x * sn[i]));
+        for (int i = 0; i < kVec; ++i) {
+            Vec<T, kVec>& v = i < kVec / 2 ? va : vb;
+            const int at = i < kVec / 2 ? 2 * i : 2 * i - kVec;
+            const float x = v.get(at), y = v.get(at + 1);
+            v.set2(at, fmaf(x, cs[i], -(y * sn[i])), fmaf(y, cs[i], x * sn[i]));
+        }
+    } else {
+        constexpr int kStep = kVec > 1 ? 2 : 1;
+#pragma unroll
+        for (int i = 0; i < kVec; i += kStep) {
+            float x[2] = {0.0f, 0.0f}, y[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int k = 0; k < kStep; ++k) {
+                const float p = va.get(i + k), q = vb.get(i + k);
+                x[k] = fmaf(p, cs[i + k], -(q * sn[i + k]));
+                y[k] = fmaf(q, cs[i + k], p * sn[i + k]);
+            }
+            va.set2(i, x[0], x[1]);
+            vb.set2(i, y[0], y[1]);
         }
     }
 }
@@ -115,7 +162,7 @@ struct RotaryArgs {
 };
 
 template <typename T, int kVec, bool kInterleaved>
-__global__ void __launch_bounds__(kRThreads) rotary_kernel(const RotaryArgs a) {
+__global__ void __launch_bounds__(kRThreads, kRBlocks) rotary_kernel(const RotaryArgs a) {
     grid_dep_launch_dependents();
     const int local = static_cast<int>(fast_div(a.rot.div_groups, threadIdx.x));
     const int group = static_cast<int>(threadIdx.x) - local * a.rot.groups;
@@ -138,8 +185,8 @@ __global__ void __launch_bounds__(kRThreads) rotary_kernel(const RotaryArgs a) {
             for (int u = 0; u < kRUnroll; ++u) {
                 if (h0 + u >= h_hi) break;
                 const T* p = x + (h0 + u) * a.xs[1];
-                va[u] = *reinterpret_cast<const V*>(p + col.a);
-                if (col.has_b) vb[u] = *reinterpret_cast<const V*>(p + col.b);
+                va[u].load(p + col.a);
+                if (col.has_b) vb[u].load(p + col.b);
             }
             if (!have) {  // (under the first loads)
                 angles<kVec>(a.rot, group, position, cs, sn);
@@ -150,8 +197,8 @@ __global__ void __launch_bounds__(kRThreads) rotary_kernel(const RotaryArgs a) {
                 if (h0 + u >= h_hi) break;
                 if (col.turns) turn<T, kVec, kInterleaved>(va[u], vb[u], cs, sn);
                 T* p = y + (h0 + u) * a.ys[1];
-                *reinterpret_cast<V*>(p + col.a) = va[u];
-                if (col.has_b) *reinterpret_cast<V*>(p + col.b) = vb[u];
+                va[u].store(p + col.a);
+                if (col.has_b) vb[u].store(p + col.b);
             }
         }
     }
@@ -182,7 +229,7 @@ __device__ __forceinline__ int sequence_of(const int* cu, int batch, int token) 
 }
 
 template <typename T, int kVec, bool kInterleaved>
-__global__ void __launch_bounds__(kRThreads) append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(kRThreads, kRBlocks) append_kernel(const AppendArgs a) {
     __shared__ int cu[kSeqStage];
     grid_dep_launch_dependents();
     const int local = static_cast<int>(fast_div(a.rot.div_groups, threadIdx.x));
@@ -230,8 +277,8 @@ __global__ void __launch_bounds__(kRThreads) append_kernel(const AppendArgs a) {
             if (r >= r_hi) break;
             const T* p = r < a.heads ? q + r * a.qs[1]
                          : r < a.heads + a.heads_k ? k + (r - a.heads) * a.ks[1] : v + (r - a.heads - a.heads_k) * a.vs[1];
-            va[u] = *reinterpret_cast<const V*>(p + col.a);
-            if (col.has_b) vb[u] = *reinterpret_cast<const V*>(p + col.b);
+            va[u].load(p + col.a);
+            if (col.has_b) vb[u].load(p + col.b);
         }
         if (!have && r_lo < a.heads + a.heads_k) {
             angles<kVec>(a.rot, group, position, cs, sn);
@@ -245,8 +292,8 @@ __global__ void __launch_bounds__(kRThreads) append_kernel(const AppendArgs a) {
             T* p = r < a.heads ? q_out + r * a.qos[1]
                    : r < a.heads + a.heads_k ? k_to + (r - a.heads) * a.kps[1] : v_to + (r - a.heads - a.heads_k) * a.vps[1];
             if (r < a.heads || to_page) {
-                *reinterpret_cast<V*>(p + col.a) = va[u];
-                if (col.has_b) *reinterpret_cast<V*>(p + col.b) = vb[u];
+                va[u].store(p + col.a);
+                if (col.has_b) vb[u].store(p + col.b);
             }
         }
     }
