@@ -14,7 +14,7 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libfa_b200.so")
 SOURCES = ["fa_api.cu", "fa_fwd_tiled.cu", "fa_decode.cu", "fa_aux.cu", "fa_static_scratch.cu", "fa_ring.cu", "fa_rotary.cu", "fa_paged.cu", "fa_paged_decode.cu", "fa_paged_tiled.cu"]
-HEADERS = ["fa_internal.h", "fa_paged.h", "paged_plan.cuh", "paged_kernels.h", "paged_merge.cuh", "decode_mma.cuh", "tiled_mma.cuh", "sm100_ptx.cuh", "philox.cuh", os.path.join("..", "..", "include", "fa_b200.h")]
+HEADERS = ["fa_internal.h", "fa_paged.h", "paged_plan.cuh", "paged_kernels.h", "paged_merge.cuh", "paged_parts.cuh", "decode_mma.cuh", "tiled_mma.cuh", "sm100_ptx.cuh", "philox.cuh", os.path.join("..", "..", "include", "fa_b200.h")]
 # units of compilation (source, object, flags), longest first: the tiled kernels once for each head dimension and number of query
 # tiles a CTA (in one unit they take ptxas two minutes)
 UNITS = [("fa_fwd_tiled.cu", f"fa_fwd_tiled_{d}_{nq}.o", [f"-DFA_TILED_D={d}", f"-DFA_TILED_NQ={nq}"])

@@ -15,9 +15,13 @@ namespace fa {
 
 namespace {
 
-// A part is not worth starting for fewer tiles than kMinShare; launches of more than one wave are cut into kPagedWaves of parts, which
-// are no shorter than kLongShare.
+// A part is not worth starting for fewer tiles than min_share; launches of more than one wave are cut into `waves` of parts, which are no
+// shorter than long_share.
 constexpr int kMinShare = 4, kLongShare = 24, kPagedWaves = 3;
+// The decode kernel's: a megabyte of K and V at least (kDecodeLongShare tiles of 128 columns; 64 sequences of 100 .. 8192 keys, 8 K/V
+// heads of 128 columns: 82 us, with 8 tiles 84, with 24 tiles 88; 24 sequences of 500 .. 4000 keys, 16 heads of 64 columns: 49 us with
+// 32 tiles, 54 with 16), and the tiles a CTA up to which a launch is one wave (4 sequences of 98304 .. 131072 keys: 298 us, in waves 309).
+constexpr int kDecodeMinShare = 2, kDecodeLongShare = 16, kDecodeWaves = 4, kDecodeOneWave = 128;
 
 int check_fwd(const fa_paged_fwd_params* p) {
     if (!p || !p->q || !p->o) return FA_ERR_INVALID_ARG;
@@ -50,10 +54,11 @@ struct PagedLaunch {
     int query_tiles;           // tiled kernel: of a block
     int rows;                  // of a block
     int slots;                 // CTAs that run at once
+    int min_share, long_share, waves;
     int wide;                  // columns of a partial row: head_dim rounded up
     long long items;           // at most so many blocks of rows there are, over all K/V heads
     long long grid, partials;
-    size_t o_bytes, ml_bytes, bytes;  // workspace: partial rows, their maxima and sums, and all
+    size_t count_bytes, ml_bytes, o_bytes, bytes;  // workspace: counts of parts, maxima and sums of partial rows, the rows, and all
 };
 
 PagedLaunch plan_launch(const fa_paged_fwd_params* p, int sms) {
@@ -65,21 +70,25 @@ PagedLaunch plan_launch(const fa_paged_fwd_params* p, int sms) {
     l.columns = rows == 1 ? 1 : rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 ? 16 : 0;
     l.query_tiles = l.columns ? 0 : rows <= tile_rows ? 1 : 2;
     l.rows = l.columns ? l.columns : l.query_tiles * tile_rows;
-    l.slots = (l.query_tiles == 2 ? 1 : 2) * sms;
     l.wide = c.head_dim <= 64 ? 64 : 128;
+    l.slots = (l.query_tiles == 2 ? 1 : 2) * sms;
     l.items = c.heads * (c.cu_seqlens_q ? (p->tokens * group + static_cast<long long>(c.batch) * (l.rows - 1)) / l.rows
                                         : static_cast<long long>(c.batch) * ((group + l.rows - 1) / l.rows));
     const long long slots = l.slots;
     const long long tiles = (static_cast<long long>(c.table_width) * c.page_size + kTile - 1) / kTile;
-    const long long parts = (tiles + kMinShare - 1) / kMinShare;  // of one item
-    if (parts > 1) {
-        // (items longer than the share are cut into less than twice what the shares are)
-        l.partials = std::min(2LL * kPagedWaves * slots, l.items * parts);
-    }
-    l.grid = l.items + (parts > 1 ? std::min(kPagedWaves * slots, l.items * (parts - 1)) : 0);
-    l.o_bytes = (static_cast<size_t>(l.partials) * l.rows * l.wide * sizeof(float) + 255) & ~static_cast<size_t>(255);
-    l.ml_bytes = (static_cast<size_t>(l.partials) * l.rows * sizeof(float2) + 255) & ~static_cast<size_t>(255);
-    l.bytes = l.o_bytes + l.ml_bytes + ((static_cast<size_t>(l.partials) * 8 + 255) & ~static_cast<size_t>(255));
+    l.min_share = l.columns ? kDecodeMinShare : kMinShare;
+    l.long_share = l.columns ? kDecodeLongShare * (128 / l.wide) : kLongShare;
+    l.waves = l.columns ? kDecodeWaves : kPagedWaves;
+    const long long parts = (tiles + l.min_share - 1) / l.min_share;  // of one item
+    // (items longer than the share are cut into less than twice what the shares are; a length beyond the table's is cut like any other)
+    if (parts > 1) l.partials = 2LL * l.waves * slots;
+    l.grid = l.items + (parts > 1 ? l.waves * slots : 0);
+    auto room = [](size_t bytes) { return (bytes + 255) & ~static_cast<size_t>(255); };
+    // (the counts lie in the same place whatever the call: no count of one may be a partial row of another)
+    l.count_bytes = room(2 * std::max(kPagedWaves, kDecodeWaves) * 2 * sms * sizeof(unsigned long long));
+    l.ml_bytes = room(static_cast<size_t>(l.partials) * l.rows * sizeof(float2));
+    l.o_bytes = room(static_cast<size_t>(l.partials) * l.rows * l.wide * sizeof(float));
+    if (l.partials > 0) l.bytes = l.count_bytes + l.ml_bytes + l.o_bytes;
     return l;
 }
 
@@ -198,9 +207,10 @@ int fa_paged_fwd(const fa_paged_fwd_params* p) {
     a.plan.window_left = p->window_left < kMostKeys / 2 ? p->window_left : -1;
     a.plan.window_right = p->window_right < kMostKeys / 2 ? p->window_right : -1;
     a.plan.slots = l.slots;
-    a.plan.min_share = kMinShare;
-    a.plan.long_share = kLongShare;
-    a.plan.waves = kPagedWaves;
+    a.plan.min_share = l.min_share;
+    a.plan.long_share = l.long_share;
+    a.plan.waves = l.waves;
+    a.plan.one_wave = kDecodeOneWave;
     a.plan.partials = static_cast<int>(l.partials);
     a.div_group = make_fastdiv(static_cast<uint32_t>(a.plan.group));
     a.q = p->q;
@@ -221,9 +231,10 @@ int fa_paged_fwd(const fa_paged_fwd_params* p) {
     a.o_is_fp32 = p->o_dtype == FA_DTYPE_FP32;
     a.status = p->status;
     if (l.bytes > 0) {
-        a.o_partial = static_cast<float*>(p->workspace);
-        a.ml_partial = reinterpret_cast<float2*>(static_cast<char*>(p->workspace) + l.o_bytes);
-        a.counts = reinterpret_cast<unsigned long long*>(static_cast<char*>(p->workspace) + l.o_bytes + l.ml_bytes);
+        char* room = static_cast<char*>(p->workspace);
+        a.counts = reinterpret_cast<unsigned long long*>(room);
+        a.ml_partial = reinterpret_cast<float2*>(room + l.count_bytes);
+        a.o_partial = reinterpret_cast<float*>(room + l.count_bytes + l.ml_bytes);
     }
     cudaStream_t stream = static_cast<cudaStream_t>(p->stream);
     const bool bf16 = c.dtype == FA_DTYPE_BF16;

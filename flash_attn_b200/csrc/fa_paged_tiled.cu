@@ -536,8 +536,8 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             }
             __syncwarp();
         }
-        if (split && last_to_come<NQ * 128>(a, w, reinterpret_cast<volatile int*>(smem_gen + C::kSmemMisc + 12)))
-            merge_parts<D, kBf16, NQ * 4>(a, w, token0 * a.plan.group, min(a.plan.rows, (w.n - token0) * a.plan.group), warp);
+        if (split && last_to_come<NQ * 128>(a, w.slot, w.parts, reinterpret_cast<volatile int*>(smem_gen + C::kSmemMisc + 12)))
+            merge_parts<D, kBf16, NQ * 4, 4>(a, w.slot, w.parts, w.head, w.first, token0 * a.plan.group, min(a.plan.rows, (w.n - token0) * a.plan.group), warp);
     }
 
     if (fail != 0) {

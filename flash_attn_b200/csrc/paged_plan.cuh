@@ -25,6 +25,7 @@ struct PagedPlan {
     int min_share;        // tiles that a part is worth starting for
     int long_share;       // of launches of more than one wave: parts are no shorter than this
     int waves;            // and shares no shorter than this part of a slot's tiles
+    int one_wave;         // decode kernel: tiles a slot up to which all parts are to run at once
     int partials;         // parts of split items that there is room for (0: nothing is split)
 };
 
@@ -294,16 +295,21 @@ __device__ __forceinline__ bool find_work(const PagedPlan& p, PlanScratch& sm, i
 // was never used) counts as none come yet, and the last of the parts leaves none come for the next launch.
 constexpr unsigned long long kCountMark = 0x9d3f6ba817c5ull << 16;
 
-// Whether this CTA is the last of its item (one thread; the CTA's partial rows are visible to the device).
+// Whether this CTA is the last of its item (one thread, to whom the CTA's partial rows are visible; they are to the others' after).
 __device__ __forceinline__ bool count_in(unsigned long long* count, int parts) {
-    unsigned long long seen = *reinterpret_cast<volatile unsigned long long*>(count);
-    for (;;) {  // (ends: a failed exchange is another part's success)
-        const unsigned come = (seen & ~0xffffull) == kCountMark ? static_cast<unsigned>(seen & 0xffffull) : 0u;
-        const bool last = come + 1 >= static_cast<unsigned>(parts);
-        const unsigned long long was = atomicCAS(count, seen, kCountMark | (last ? 0u : come + 1));
-        if (was == seen) return last;
-        seen = was;
+    __threadfence();
+    unsigned long long was = atomicAdd(count, 1ull);
+    while ((was & ~0xffffull) != kCountMark) {  // not a count: whoever makes it one is the first to come, the others add themselves again
+        const unsigned long long seen = *reinterpret_cast<volatile unsigned long long*>(count);
+        if ((seen & ~0xffffull) == kCountMark) was = atomicAdd(count, 1ull);
+        else if (atomicCAS(count, seen, kCountMark | 1ull) == seen) was = kCountMark;  // (ends: a failed exchange is another part's doing)
     }
+    const bool last = static_cast<int>(was & 0xffffull) + 1 == parts;
+    if (last) {
+        *reinterpret_cast<volatile unsigned long long*>(count) = kCountMark;
+        __threadfence();
+    }
+    return last;
 }
 #endif
 

@@ -116,6 +116,27 @@ __device__ __forceinline__ float4 ld_shared_f32x4_if(uint32_t addr, bool take) {
     return v;
 }
 
+// ---------------------------------------------------------------- cluster launch control
+// Asks for a CTA of this grid that has not started: it then never does, and the caller does its work.  The answer, 16 bytes, is
+// counted on `bar`.  Not to be asked again once the answer was that there is none.
+__device__ __forceinline__ void launch_take(uint32_t answer, uint32_t bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer), "r"(bar) : "memory");
+}
+// Its index, or -1.
+__device__ __forceinline__ int launch_taken(uint32_t answer) {
+    uint32_t have, x = 0;
+    asm volatile(
+        "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\t"
+        "ld.shared.b128 h, [%2];\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t}"
+        : "=r"(have), "+r"(x)
+        : "r"(answer)
+        : "memory");
+    return have ? static_cast<int>(x) : -1;
+}
+
 // ---------------------------------------------------------------- fences
 __device__ __forceinline__ void fence_proxy_async_smem() {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -182,6 +203,16 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
         ::"r"(dst), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
         : "memory");
 }
+
+// 16 bytes global -> shared past L1, or 16 zero bytes where `take` is false (nothing is read then).
+__device__ __forceinline__ void copy16_async_if(uint32_t dst, const void* src, bool take) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
+}
+// Arrives on `bar` once the copies that this thread has issued so far have landed.
+__device__ __forceinline__ void copies_arrive(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void copies_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // ---------------------------------------------------------------- TMEM
 // All three are warp-collective (.sync.aligned): call with a converged warp.
