@@ -1,6 +1,6 @@
 // Attention of chunks of new tokens over a paged K/V cache: tensor-bound.
 //
-// One CTA = one part of the keys of one block of rows (paged_plan.cuh), NQ query tiles of 128 rows.  A row is a token and a query head:
+// A CTA walks parts of the keys of blocks of rows, one behind the other (paged_parts.cuh); a block is NQ query tiles of 128 rows.  A row is a token and a query head:
 // the heads of a K/V head lie side by side in a tile (row = token * group + head, as one TMA box of Q lands), so that they share every
 // K/V tile and a few tokens fill it; where the group does not divide 128 the tile's last rows are left over.
 // The walk is the tiled kernel's for contiguous K/V: a TMA warp feeds a ring of K/V tiles, an MMA warp issues S = Q K^T into tensor
@@ -17,6 +17,7 @@
 #include <type_traits>
 #include "paged_kernels.h"
 #include "paged_merge.cuh"
+#include "paged_parts.cuh"
 #include "paged_plan.cuh"
 #include "sm100_ptx.cuh"
 #include "tiled_mma.cuh"
@@ -33,6 +34,7 @@ namespace {
 constexpr float kRescaleThreshold = 8.0f;  // log2 units: rescale O only when the max grew by > 2^8
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kSegs = 4;  // parts that the producer may have handed on before the first of them is done
 
 // Column pairs that take the polynomial exp2, a quarter of them (see the tiled kernel for contiguous K/V).
 __host__ __device__ constexpr uint32_t poly_mask(int d, bool alibi) { return alibi ? 0x11u : d == 128 ? 0x88u : 0x81u; }
@@ -81,8 +83,8 @@ struct TCfg {
     // Registers: the CTA owns kThreads * kRegsLaunch from launch on (168 a thread under __launch_bounds__(384, 1), 128 under (256, 2));
     // an increase that asks for more than the helper warps released would wait for ever.
     static constexpr int kRegsLaunch = NQ == 2 ? 168 : 128;
-    static constexpr int kRegsHelper = NQ == 2 ? 56 : 48;
-    static constexpr int kRegsSoftmax = NQ == 2 ? 224 : 208;
+    static constexpr int kRegsHelper = NQ == 2 ? 72 : 48;
+    static constexpr int kRegsSoftmax = NQ == 2 ? 216 : 208;
     static_assert(NQ * 128 * kRegsSoftmax + 128 * kRegsHelper <= kThreads * kRegsLaunch, "register hand-over exceeds the CTA's allocation");
     static constexpr int kProducerWarp = NQ * 4, kMmaWarp = NQ * 4 + 1;
     static constexpr int kStages = (D == 64) ? (NQ == 2 ? 3 : 2) : (NQ == 2 ? 2 : 1);
@@ -93,11 +95,13 @@ struct TCfg {
     static constexpr int kSmemQ = 0;
     static constexpr int kSmemK = NQ * kTileBytes;
     static constexpr int kSmemV = kSmemK + kStages * kTileBytes;
-    static constexpr int kSmemBar = kSmemV + kStages * kTileBytes;
-    static constexpr int kNumBars = 1 + 2 * NQ + 4 * kStages;
-    static constexpr int kSmemMisc = kSmemBar + 8 * kNumBars;  // tensor-memory address, abort flag, bad page
-    static constexpr int kSmemPlan = (kSmemMisc + 16 + 15) / 16 * 16;
-    static constexpr int kSmemBytes = kSmemPlan + static_cast<int>(sizeof(PlanScratch)) + 1024;  // + alignment slack
+    static constexpr int kStageCols = NQ == 2 ? 32 : 16;               // columns of its output rows that a warp has in shared memory at once
+    static constexpr int kSmemRows = kSmemV + kStages * kTileBytes;
+    static constexpr int kSmemBar = kSmemRows + NQ * 4 * 32 * kStageCols * 4;
+    static constexpr int kNumBars = 2 + 2 * NQ + 4 * kStages + 2 * kSegs + 1;
+    static constexpr int kSmemMisc = (kSmemBar + 8 * kNumBars + 15) / 16 * 16;  // tensor-memory address, abort flag, last part's flag
+    static constexpr int kSmemSegs = kSmemMisc + 16 + 4 * kSegs;                // (which parts met a bad page;) PagedSeg[kSegs], a taken CTA
+    static constexpr int kSmemBytes = kSmemSegs + kSegs * static_cast<int>(sizeof(PagedSeg)) + 16 + 1024;  // + alignment slack
     static_assert(kSmemBytes <= (NQ == 2 ? 232448 : 115712), "one or two CTAs per SM");
 };
 
@@ -117,17 +121,23 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     const uint32_t bar_k_empty = bar_k_full + 8 * C::kStages;  // [kStages]
     const uint32_t bar_v_full = bar_k_empty + 8 * C::kStages;  // [kStages]
     const uint32_t bar_v_empty = bar_v_full + 8 * C::kStages;  // [kStages]
+    const uint32_t bar_q_free = bar_v_empty + 8 * C::kStages;
+    const uint32_t bar_taken = bar_q_free + 8;
+    const uint32_t bar_seg_full = bar_taken + 8;               // [kSegs]
+    const uint32_t bar_seg_free = bar_seg_full + 8 * kSegs;    // [kSegs]
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem_gen + C::kSmemMisc);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem_gen + C::kSmemMisc + 4);
-    volatile int* bad_page = reinterpret_cast<volatile int*>(smem_gen + C::kSmemMisc + 8);
+    volatile int* last_flag = reinterpret_cast<volatile int*>(smem_gen + C::kSmemMisc + 8);
+    volatile int* bad_seg = reinterpret_cast<volatile int*>(smem_gen + C::kSmemMisc + 16);  // [kSegs]: the part met a bad page
+    PagedSeg* segs = reinterpret_cast<PagedSeg*>(smem_gen + C::kSmemSegs);
+    const uint32_t taken = smem_base + C::kSmemSegs + kSegs * static_cast<int>(sizeof(PagedSeg));
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     grid_dep_launch_dependents();
     if (warp == C::kProducerWarp) {
-        if (lane < C::kNumBars) mbar_init(bar0 + 8 * lane, 1);
+        if (lane < C::kNumBars) mbar_init(bar0 + 8 * lane, bar0 + 8 * lane >= bar_seg_free ? 1 + NQ * 4 : 1);
         if (lane == 0) {
             *abort_flag = 0;
-            *bad_page = 0;
             tma_prefetch_desc(&tmap_q);
             tma_prefetch_desc(&tmap_k);
             tma_prefetch_desc(&tmap_v);
@@ -136,105 +146,138 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         if (lane == 0) mbar_fence_init();
     }
     grid_dep_wait();  // every thread, before its first global access
-    PagedWork w;
-    if (!find_work<C::kThreads>(a.plan, *reinterpret_cast<PlanScratch*>(smem_gen + C::kSmemPlan), static_cast<int>(blockIdx.x), &w))
-        return;
-
-    // ---- the block's query tiles, and the tiles of keys of this part
+    long long tiles_in_all = 0;
+    if (a.plan.seq.batch > kWarpSeqs) {
+        long long sum = 0;
+        for (int b = threadIdx.x; b < a.plan.seq.batch; b += C::kThreads) {
+            const int2 x = blocks_and_tiles(a.plan, seq_span(a.plan.seq, b));
+            sum += static_cast<long long>(x.x) * x.y;
+        }
+        sum = sum_all(sum);
+        long long* sums = reinterpret_cast<long long*>(smem_gen + C::kSmemRows);
+        if (lane == 0) sums[warp] = sum;
+        __syncthreads();
+        for (int i = 0; i < C::kThreads / 32; ++i) tiles_in_all += sums[i];
+        tiles_in_all *= a.plan.heads_k;
+    }
     const int tile_tokens = a.tile_tokens, tile_rows = tile_tokens * a.plan.group;
-    const int token0 = w.blk * NQ * tile_tokens;  // first token of the block inside the sequence
-    const int p_first = w.keys - w.n;             // position of the sequence's first new token
-    struct Range { int lo, hi; } range[NQ];
-    int vis_lo = 0x7fffffff, vis_hi = 0, lo = 0x7fffffff, hi = 0;
-#pragma unroll
-    for (int i = 0; i < NQ; ++i) {
-        const int t0 = token0 + i * tile_tokens, t1 = min(t0 + tile_tokens, w.n) - 1;
+    // The tiles of a part that query tile i walks: [lo, hi).
+    struct Range { int lo, hi; };
+    auto range_of = [&](const PagedSeg& g, int token0, int i) -> Range {
+        const int t0 = token0 + i * tile_tokens, t1 = min(t0 + tile_tokens, g.n) - 1;
         int l = 0, h = 0;
-        if (t1 >= t0) visible_keys(a.plan, w.keys, p_first + t0, p_first + t1, &l, &h);
-        range[i] = {l / kTile, h > l ? (h + kTile - 1) / kTile : l / kTile};
-        if (h > l) {
-            vis_lo = min(vis_lo, l);
-            vis_hi = max(vis_hi, h);
-            lo = min(lo, range[i].lo);
-            hi = max(hi, range[i].hi);
-        }
-    }
-    const int n_all = hi > lo ? hi - lo : 0, lo_all = hi > lo ? lo : 0;
-    if (w.parts > 1) {
-        int p_lo, p_hi;
-        part_of(n_all, w.part, w.parts, &p_lo, &p_hi);
-        p_lo += lo_all;
-        p_hi += lo_all;
-        lo = 0x7fffffff;
-        hi = 0;
-#pragma unroll
-        for (int i = 0; i < NQ; ++i) {
-            range[i].lo = max(range[i].lo, p_lo);
-            range[i].hi = max(min(range[i].hi, p_hi), range[i].lo);
-            if (range[i].hi > range[i].lo) {
-                lo = min(lo, range[i].lo);
-                hi = max(hi, range[i].hi);
-            }
-        }
-    }
-    const int n_union = hi > lo ? hi - lo : 0;  // KV tiles of this CTA: [lo, hi)
-
-    // ---- set-up: loads of Q and the first K/V tiles, tensor memory
-    const PageLane page_box = page_lane<C::kBoxes>(a, lane);
-    const int* table = a.page_table + w.b * a.table_stride;
-    bool met_bad = false;
-    auto lookup = [&](int tile) { return page_lookup(a, page_box, table, tile, vis_lo, vis_hi, &met_bad); };
-    auto load = [&](bool of_k, uint32_t dst, uint32_t bar, int tile, int page) {
-        if (__any_sync(0xffffffffu, met_bad) && lane == 0) *bad_page = 1;  // (before what the readers' barriers wait for)
-        page_load<C::kBoxes>(a, of_k ? a.k_box : a.v_box, page_box, of_k ? &tmap_k : &tmap_v, dst, bar, tile, w.head, page);
+        if (t1 >= t0) visible_keys(a.plan, g.keys, g.keys - g.n + t0, g.keys - g.n + t1, &l, &h);
+        const int lo = max(h > l ? l / kTile : g.lo, g.lo);
+        return {lo, max(min(h > l ? (h + kTile - 1) / kTile : lo, g.lo + g.n_tiles), lo)};
     };
-    int prefilled = 0;
-    if (warp == C::kProducerWarp && n_union > 0) {
-        int page[C::kStages];
-        prefilled = min(C::kStages, n_union);
-#pragma unroll
-        for (int t = 0; t < C::kStages; ++t) page[t] = t < prefilled ? lookup(hi - 1 - t) : -1;
-        int q_tiles = 0;
-#pragma unroll
-        for (int i = 0; i < NQ; ++i) q_tiles += token0 + i * tile_tokens < w.n ? 1 : 0;
-        if (lane == 0) mbar_expect_tx(bar_q_full, q_tiles * C::kBoxes * tile_rows * 128);
-        __syncwarp();
-        if (lane < q_tiles * C::kBoxes) {
-            const int i = lane / C::kBoxes, b = lane % C::kBoxes;
-            tma_load_4d(sQ + i * C::kTileBytes + b * (kTile * 128), &tmap_q, bar_q_full, b * 64, 0, w.head, w.first + token0 + i * tile_tokens);
+    auto token_of = [&](const PagedSeg& g) { return static_cast<int>(fast_div(a.div_group, static_cast<uint32_t>(g.row0))); };
+    // Parts are handed on and freed whatever else gives up: every warp walks all parts of the CTA, so that the named barriers are
+    // posted and met in full, and the CTA's parts are counted in.  (No flag ends these waits; each is bounded all the same.)
+    auto wait_part = [&](uint32_t bar, uint32_t parity) -> bool {
+        for (int i = 0; i < 8; ++i) {
+            volatile int own = 0;
+            if (mbar_wait_warp(bar, parity, &own)) return true;
         }
-#pragma unroll
-        for (int t = 0; t < C::kStages; ++t) {  // KV tiles are walked from the last to the first
-            if (t >= prefilled) break;
-            load(true, sK + t * C::kTileBytes, bar_k_full + 8 * t, hi - 1 - t, page[t]);
-            load(false, sV + t * C::kTileBytes, bar_v_full + 8 * t, hi - 1 - t, page[t]);
-        }
-    }
-    if (warp == C::kMmaWarp && n_union > 0) {
+        return false;
+    };
+
+    // ---- set-up: tensor memory
+    if (warp == C::kMmaWarp) {
         tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), C::kTmemCols);
         tmem_relinquish();
     }
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
-    const uint32_t tmem_base = (n_union > 0) ? *tmem_slot : 0u;
+    const uint32_t tmem_base = *tmem_slot;
 
     int fail = 0;
     if (warp >= NQ * 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsHelper));
-        if (n_union > 0 && warp == C::kProducerWarp) {
-            // ======================= TMA producer ===================================
-            for (int t = prefilled; t < n_union; ++t) {
-                const int st = t % C::kStages;
-                const uint32_t ph = (t / C::kStages) & 1;
-                const int tile = hi - 1 - t, page = lookup(tile);
-                if (!mbar_wait_warp(bar_k_empty + 8 * st, ph ^ 1, abort_flag)) { fail = 1; break; }
-                load(true, sK + st * C::kTileBytes, bar_k_full + 8 * st, tile, page);
-                if (!mbar_wait_warp(bar_v_empty + 8 * st, ph ^ 1, abort_flag)) { fail = 2; break; }
-                load(false, sV + st * C::kTileBytes, bar_v_full + 8 * st, tile, page);
+        if (warp == C::kProducerWarp) {
+            // ======================= producer =======================================
+            const PageLane page_box = page_lane<C::kBoxes>(a, lane);
+            PartLine line;
+            line.start(a.plan, lane, tiles_in_all);
+            int index = static_cast<int>(blockIdx.x), asked = 0, answered = 0;  // the CTA whose part is next; -1: there is none
+            auto ask = [&] {
+                if (asked > answered || index < 0 || fail != 0) return;
+                if (lane == 0) {
+                    mbar_expect_tx(bar_taken, 16);
+                    launch_take(taken, bar_taken);
+                }
+                ++asked;
+            };
+            auto answer = [&] {
+                index = -1;
+                if (asked == answered) return;  // (not asked: something gave up)
+                if (!wait_part(bar_taken, answered & 1)) return;
+                index = launch_taken(taken);
+                fence_proxy_async_smem();  // (read before the next answer is written)
+                __syncwarp();
+                ++answered;
+            };
+            int tt = 0, parts_with_tiles = 0;
+            for (int nth = 0;; ++nth) {
+                if (nth > 0) {
+                    ask();
+                    answer();
+                }
+                const int at = nth % kSegs;
+                if (nth >= kSegs && !wait_part(bar_seg_free + 8 * at, (nth / kSegs - 1) & 1)) { fail = 3; break; }
+                PagedSeg g;
+                const bool have = index >= 0 && line.find(a.plan, a.div_group, index, lane, &g);
+                if (!have) g.n_rows = 0;
+                if (lane == 0) {
+                    segs[at] = g;
+                    bad_seg[at] = 0;
+                    mbar_arrive(bar_seg_full + 8 * at);
+                }
+                __syncwarp();
+                if (!have) {
+                    while (index >= 0) {  // CTAs behind the last part need not start
+                        ask();
+                        answer();
+                    }
+                    break;
+                }
+                if (g.n_tiles == 0) continue;
+                const int* table = a.page_table + g.b * a.table_stride;
+                bool met_bad = false;
+                auto lookup = [&](int tile) { return page_lookup(a, page_box, table, tile, g.vis_lo, g.vis_hi, &met_bad); };
+                auto load = [&](bool of_k, uint32_t dst, uint32_t bar, int tile, int page) {
+                    page_load<C::kBoxes>(a, of_k ? a.k_box : a.v_box, page_box, of_k ? &tmap_k : &tmap_v, dst, bar, tile, g.head, page);
+                };
+                const int token0 = token_of(g), hi = g.lo + g.n_tiles;
+                for (int t = 0; t < g.n_tiles && fail == 0; ++t, ++tt) {  // KV tiles are walked from the last to the first
+                    const int st = tt % C::kStages;
+                    const uint32_t ph = (tt / C::kStages) & 1;
+                    const int tile = hi - 1 - t, page = lookup(tile);
+                    if (__any_sync(0xffffffffu, met_bad) && lane == 0) bad_seg[at] = 1;  // (before what the readers' barriers wait for)
+                    if (!mbar_wait_warp(bar_k_empty + 8 * st, ph ^ 1, abort_flag)) { fail = 1; break; }
+                    load(true, sK + st * C::kTileBytes, bar_k_full + 8 * st, tile, page);
+                    if (t == 0) {
+                        if (parts_with_tiles > 0 && !mbar_wait_warp(bar_q_free, (parts_with_tiles - 1) & 1, abort_flag)) { fail = 1; break; }
+                        ++parts_with_tiles;
+                        int q_tiles = 0;
+#pragma unroll
+                        for (int i = 0; i < NQ; ++i) q_tiles += token0 + i * tile_tokens < g.n ? 1 : 0;
+                        if (lane == 0) mbar_expect_tx(bar_q_full, q_tiles * C::kBoxes * tile_rows * 128);
+                        __syncwarp();
+                        if (lane < q_tiles * C::kBoxes) {
+                            const int i = lane / C::kBoxes, b = lane % C::kBoxes;
+                            tma_load_4d(sQ + i * C::kTileBytes + b * (kTile * 128), &tmap_q, bar_q_full, b * 64, 0, g.head, g.first + token0 + i * tile_tokens);
+                        }
+                    }
+                    if (t + 1 == g.n_tiles) ask();  // (the answer is here when it is needed)
+                    if (!mbar_wait_warp(bar_v_empty + 8 * st, ph ^ 1, abort_flag)) { fail = 2; break; }
+                    load(false, sV + st * C::kTileBytes, bar_v_full + 8 * st, tile, page);
+                }
+                if (__any_sync(0xffffffffu, met_bad) && lane == 0 && a.status != nullptr) atomicExch(a.status, FA_STATUS_PAGE);
+                if (fail != 0 && lane == 0) *abort_flag = 1;
+                __syncwarp();
             }
-            if (__any_sync(0xffffffffu, met_bad) && lane == 0 && a.status != nullptr) atomicExch(a.status, FA_STATUS_PAGE);
-        } else if (n_union > 0 && warp == C::kMmaWarp) {
+        } else if (warp == C::kMmaWarp) {
             // ======================= MMA issuer =====================================
             const bool leader = elect_one();
             constexpr uint32_t idesc_qk = make_idesc_f16(kTile, kTile, kBf16, false);
@@ -247,66 +290,76 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             const uint32_t k_jump = half_bytes / 16 - 6, v_step = eight_bytes / 8;
             auto issue_s = [&](int i, int st) {
                 issue_qk<D>(tmem_base + i * kTile, q_lo + ((i * C::kTileBytes) >> 4), k_lo + ((st * C::kTileBytes) >> 4), q_hi, kv_hi, k_jump, idesc_qk);
+                umma_commit(bar_s_full + 8 * i);
             };
-            auto active = [&](int i, int tile) { return tile >= range[i].lo && tile < range[i].hi; };
-            do {
-                if (!mbar_wait_warp(bar_q_full, 0, abort_flag)) { fail = 3; break; }
-                if (!mbar_wait_warp(bar_k_full, 0, abort_flag)) { fail = 4; break; }
-                tc_fence_after_sync();
-                if (leader) {
+            // (after a wait gave up: nothing more is issued, and the named barriers are met as ever)
+            auto ready = [&](uint32_t bar, uint32_t parity, int code) {
+                if (fail == 0 && !mbar_wait_warp(bar, parity, abort_flag)) fail = code;
+            };
+            int tt = 0, parts_with_tiles = 0;
+            for (int nth = 0;; ++nth) {
+                const int at = nth % kSegs;
+                if (!wait_part(bar_seg_full + 8 * at, (nth / kSegs) & 1)) { fail = 3; break; }
+                const PagedSeg& g = segs[at];
+                if (g.n_rows == 0) break;
+                const int n_union = g.n_tiles, hi = g.lo + g.n_tiles, vis_lo = g.vis_lo, vis_hi = g.vis_hi;
+                Range range[NQ];
 #pragma unroll
-                    for (int i = 0; i < NQ; ++i) {
-                        if (active(i, hi - 1)) {
-                            issue_s(i, 0);
-                            umma_commit(bar_s_full + 8 * i);
-                        }
+                for (int i = 0; i < NQ; ++i) range[i] = range_of(g, token_of(g), i);
+                auto active = [&](int i, int tile) { return tile >= range[i].lo && tile < range[i].hi; };
+                if (n_union > 0) {
+                    ready(bar_q_full, parts_with_tiles & 1, 4);
+                    ++parts_with_tiles;
+                    ready(bar_k_full + 8 * (tt % C::kStages), (tt / C::kStages) & 1, 5);
+                    tc_fence_after_sync();
+                    if (leader && fail == 0) {
+#pragma unroll
+                        for (int i = 0; i < NQ; ++i)
+                            if (active(i, hi - 1)) issue_s(i, tt % C::kStages);
+                        umma_commit(bar_k_empty + 8 * (tt % C::kStages));
+                        if (n_union == 1) umma_commit(bar_q_free);
                     }
-                    umma_commit(bar_k_empty);
                 }
-                for (int t = 0; t < n_union && fail == 0; ++t) {
+                for (int t = 0; t < n_union; ++t, ++tt) {
                     const int tile = hi - 1 - t;
-                    const int st = t % C::kStages;
-                    const uint32_t ph = (t / C::kStages) & 1;
-                    const int st1 = (t + 1) % C::kStages;
-                    const uint32_t ph1 = ((t + 1) / C::kStages) & 1;
+                    const int st = tt % C::kStages;
+                    const uint32_t ph = (tt / C::kStages) & 1;
+                    const int st1 = (tt + 1) % C::kStages;
+                    const uint32_t ph1 = ((tt + 1) / C::kStages) & 1;
                     const bool more = t + 1 < n_union;
-                    if (!mbar_wait_warp(bar_v_full + 8 * st, ph, abort_flag)) { fail = 6; break; }
-                    if (tile * kTile < vis_lo || tile * kTile + kTile > vis_hi) {
-                        // keys that no row of the block sees: their rows of V may hold anything
+                    ready(bar_v_full + 8 * st, ph, 6);
+                    // keys that no row of the block sees: their rows of V may hold anything
+                    if (tile * kTile < vis_lo || tile * kTile + kTile > vis_hi)
                         clear_rows<C::kBoxes>(a, sV + st * C::kTileBytes, max(vis_lo - tile * kTile, 0), min(vis_hi - tile * kTile, kTile));
-                    }
-                    if (more) {
-                        if (!mbar_wait_warp(bar_k_full + 8 * st1, ph1, abort_flag)) { fail = 7; break; }
-                    }
+                    if (more) ready(bar_k_full + 8 * st1, ph1, 7);
 #pragma unroll
                     for (int i = 0; i < NQ; ++i) {
                         if (active(i, tile)) {
                             // P V starts on the first half of P while the second half is exponentiated
                             named_sync(1 + 2 * i);
                             tc_fence_after_sync();
-                            if (leader)
+                            if (leader && fail == 0)
                                 issue_pv<0>(tmem_base + C::kTmemO + i * D, tmem_base + i * kTile, v_lo + ((st * C::kTileBytes) >> 4), kv_hi, v_step, idesc_pv,
-                                               tile < range[i].hi - 1 ? 1u : 0u);
+                                            tile < range[i].hi - 1 ? 1u : 0u);
                             named_sync(2 + 2 * i);
                             tc_fence_after_sync();
-                            if (leader) {
-                                issue_pv<kSplitSteps>(tmem_base + C::kTmemO + i * D, tmem_base + i * kTile, v_lo + ((st * C::kTileBytes) >> 4), kv_hi, v_step, idesc_pv, 1u);
+                            if (leader && fail == 0) {
+                                issue_pv<kSplitSteps>(tmem_base + C::kTmemO + i * D, tmem_base + i * kTile, v_lo + ((st * C::kTileBytes) >> 4), kv_hi, v_step,
+                                                      idesc_pv, 1u);
                                 if (tile == range[i].lo) umma_commit(bar_o_full + 8 * i);
                             }
                         }
-                        if (more && active(i, tile - 1)) {
-                            if (leader) {
-                                issue_s(i, st1);
-                                umma_commit(bar_s_full + 8 * i);
-                            }
-                        }
+                        if (more && active(i, tile - 1) && leader && fail == 0) issue_s(i, st1);
                     }
-                    if (leader) {
+                    if (leader && fail == 0) {
                         umma_commit(bar_v_empty + 8 * st);
                         if (more) umma_commit(bar_k_empty + 8 * st1);
+                        if (t + 2 == n_union) umma_commit(bar_q_free);
                     }
                 }
-            } while (false);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_seg_free + 8 * at);
+            }
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kRegsSoftmax));
@@ -314,230 +367,228 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         const int qi = warp >> 2;           // which query tile of the CTA
         const int r = threadIdx.x & 127;    // row inside the tile
         const int r_tok = static_cast<int>(fast_div(a.div_group, static_cast<uint32_t>(r)));
-        const int tok = token0 + qi * tile_tokens + r_tok;                 // token inside the sequence
-        const int head = w.head * a.plan.group + r - r_tok * a.plan.group;  // query head
-        const bool mine = r_tok < tile_tokens && tok < w.n;                // (rows left over are walked too; nobody reads them)
-        const int qpos = p_first + tok;
-        const int t_lo = qi == 0 ? range[0].lo : range[NQ - 1].lo;
-        const int n_tiles = (qi == 0 ? range[0].hi : range[NQ - 1].hi) - t_lo;
         const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t tmem_s = tmem_base + qi * kTile;          // S, 128 fp32 columns; P (16-bit, two per column) over the first half
         const uint32_t tmem_o = tmem_base + C::kTmemO + qi * D;  // O, D fp32 columns
         const uint32_t my_s_full = bar_s_full + 8 * qi, my_o_full = bar_o_full + 8 * qi;
-        float m_ref = -INFINITY;  // running max in log2 units (scaled, biased)
-        float l_sum = 0.0f;
-        float slope2 = 0.0f;
-        if constexpr (kAlibi) slope2 = mine ? a.alibi_slopes[head] * kLog2e : 0.0f;
         const float scale2 = a.scale_log2;
+        uint32_t s_phase = 0, o_phase = 0;
+        for (int nth = 0;; ++nth) {
+            const int at = nth % kSegs;
+            if (!wait_part(bar_seg_full + 8 * at, (nth / kSegs) & 1)) { fail = 10; break; }
+            const PagedSeg& g = segs[at];
+            if (g.n_rows == 0) break;
+            const int token0 = token_of(g), keys = g.keys;
+            const int tok = token0 + qi * tile_tokens + r_tok;                 // token inside the sequence
+            const int head = g.head * a.plan.group + r - r_tok * a.plan.group;  // query head
+            const bool mine = r_tok < tile_tokens && tok < g.n;                // (rows left over are walked too; nobody reads them)
+            const int qpos = keys - g.n + tok;
+            const Range range = range_of(g, token0, qi);
+            const int t_lo = range.lo, n_tiles = range.hi - t_lo;
+            float m_ref = -INFINITY;  // running max in log2 units (scaled, biased)
+            float l_sum = 0.0f;
+            float slope2 = 0.0f;
+            if constexpr (kAlibi) slope2 = mine ? a.alibi_slopes[head] * kLog2e : 0.0f;
 
-        for (int j = 0; j < n_tiles; ++j) {
-            const int cb = t_lo + n_tiles - 1 - j;  // from the last KV tile of this query tile to the first
-            const int kbase = cb * kTile;
-            // columns this row may attend to inside the tile: [c_lo, c_hi] (worked out before S arrives)
-            int c_lo = 0, c_hi = kTile - 1;
-            if (mine) {
-                c_hi = min(c_hi, w.keys - 1 - cb * kTile);
-                if (a.plan.is_causal) c_hi = min(c_hi, qpos - kbase);
-                if (a.plan.window_right >= 0) c_hi = min(c_hi, qpos + a.plan.window_right - kbase);
-                if (a.plan.window_left >= 0) c_lo = max(0, min(qpos - a.plan.window_left - kbase, kTile));
-            }
-            const bool tile_masked = __any_sync(0xffffffffu, c_lo > 0 || c_hi < kTile - 1);
-            if (fail != 0 || !mbar_wait_warp(my_s_full, j & 1, abort_flag)) {
-                // a wait gave up: keep the barrier protocol alive (the MMA warp counts on two arrivals per tile) and do nothing else
-                fail = 8;
-                named_arrive(1 + 2 * qi);
-                named_arrive(2 + 2 * qi);
-                continue;
-            }
-            tc_fence_after_sync();
+            for (int j = 0; j < n_tiles; ++j) {
+                const int cb = t_lo + n_tiles - 1 - j;  // from the last KV tile of this query tile to the first
+                const int kbase = cb * kTile;
+                // columns this row may attend to inside the tile: [c_lo, c_hi] (worked out before S arrives)
+                int c_lo = 0, c_hi = kTile - 1;
+                if (mine) {
+                    c_hi = min(c_hi, keys - 1 - cb * kTile);
+                    if (a.plan.is_causal) c_hi = min(c_hi, qpos - kbase);
+                    if (a.plan.window_right >= 0) c_hi = min(c_hi, qpos + a.plan.window_right - kbase);
+                    if (a.plan.window_left >= 0) c_lo = max(0, min(qpos - a.plan.window_left - kbase, kTile));
+                }
+                const bool tile_masked = __any_sync(0xffffffffu, c_lo > 0 || c_hi < kTile - 1);
+                if (fail != 0 || !mbar_wait_warp(my_s_full, (s_phase + j) & 1, abort_flag)) {
+                    // a wait gave up: keep the barrier protocol alive (the MMA warp counts on two arrivals per tile) and do nothing else
+                    fail = 8;
+                    named_arrive(1 + 2 * qi);
+                    named_arrive(2 + 2 * qi);
+                    continue;
+                }
+                tc_fence_after_sync();
 
-            float s[128];
-            {
-                uint32_t tmp[4][32];
+                float s[128];
+                {
+                    uint32_t tmp[4][32];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld32(tmem_s + lane_base + c * 32, tmp[c]);
-                tmem_wait_ld();
-#pragma unroll
-                for (int c = 0; c < 128; ++c) s[c] = __uint_as_float(tmp[c / 32][c % 32]);
-            }
-            if (tile_masked) {
-                // (two passes: a causal diagonal, the common case, needs only the upper bound)
-                if (__any_sync(0xffffffffu, c_hi < kTile - 1)) {
-#pragma unroll
-                    for (int c = 0; c < 128; ++c)
-                        if (c > c_hi) s[c] = -INFINITY;
-                }
-                if (__any_sync(0xffffffffu, c_lo > 0)) {
-#pragma unroll
-                    for (int c = 0; c < 128; ++c)
-                        if (c < c_lo) s[c] = -INFINITY;
-                }
-            }
-            if constexpr (kAlibi) {
-                const float dist0 = static_cast<float>(qpos - kbase);
-#pragma unroll
-                for (int c = 0; c < 128; ++c) s[c] = fmaf(-slope2, fabsf(dist0 - static_cast<float>(c)), s[c] * scale2);
-            }
-            // tile max in log2 units; without ALiBi it is taken over the raw scores and the scale folded into the exponent's FMA
-            float m_tile;
-            {
-                float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-                for (int c = 4; c < 128; c += 8) {
-                    mx[0] = max3(mx[0], s[c], s[c + 1]);
-                    mx[1] = max3(mx[1], s[c + 2], s[c + 3]);
-                    if (c + 4 < 128) {
-                        mx[2] = max3(mx[2], s[c + 4], s[c + 5]);
-                        mx[3] = max3(mx[3], s[c + 6], s[c + 7]);
-                    }
-                }
-                m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                if constexpr (!kAlibi) m_tile *= scale2;
-            }
-            // lazy rescale: keep the old reference max unless the new one is much larger
-            float m_new = m_ref, factor = 1.0f;
-            if (m_tile > m_ref + kRescaleThreshold || m_ref == -INFINITY) {
-                m_new = fmaxf(m_ref, m_tile);
-                factor = (m_ref == -INFINITY) ? 0.0f : fast_exp2(m_ref - m_new);
-            }
-            const bool rescale = (j > 0) && (m_new != m_ref);
-            if (__any_sync(0xffffffffu, rescale)) {
-                // P V of the previous tile has completed (its commit precedes s_full), so O is stable.  A row that has seen no key yet
-                // starts from zero, whatever the values of keys that it does not see have left.
-                const float f = rescale ? factor : 1.0f;
-                const uint32_t seen = rescale && m_ref == -INFINITY ? 0u : 0xffffffffu;
-#pragma unroll
-                for (int c = 0; c < D / 32; ++c) {
-                    uint32_t orow[32];
-                    tmem_ld32(tmem_o + lane_base + c * 32, orow);
+                    for (int c = 0; c < 4; ++c) tmem_ld32(tmem_s + lane_base + c * 32, tmp[c]);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) orow[i] = __float_as_uint(__uint_as_float(orow[i] & seen) * f);
-                    tmem_st32(tmem_o + lane_base + c * 32, orow);
+                    for (int c = 0; c < 128; ++c) s[c] = __uint_as_float(tmp[c / 32][c % 32]);
                 }
-            }
-            l_sum *= (m_new != m_ref) ? factor : 1.0f;
-            m_ref = m_new;
-            const float neg_m = (m_ref == -INFINITY) ? 0.0f : -m_ref;
-
-            // P = exp2(s * scale - m), rounded to the inputs' type for the tensor core; its sum is not
-            float2 acc[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
-            const float2 neg_m2 = make_float2(neg_m, neg_m);
-            const float2 scale22 = kAlibi ? make_float2(1.0f, 1.0f) : make_float2(scale2, scale2);
-            auto exp_tile = [&](auto guard_tag) {
-                constexpr bool kGuard = decltype(guard_tag)::value;  // the tile has masked (-inf) scores, for which the polynomial gives 2^-126
-                constexpr uint32_t kPolyMask = poly_mask(D, kAlibi);
+                if (tile_masked) {
+                    // (two passes: a causal diagonal, the common case, needs only the upper bound)
+                    if (__any_sync(0xffffffffu, c_hi < kTile - 1)) {
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {  // quarters of 32 columns
-                    uint32_t pr[16];
+                        for (int c = 0; c < 128; ++c)
+                            if (c > c_hi) s[c] = -INFINITY;
+                    }
+                    if (__any_sync(0xffffffffu, c_lo > 0)) {
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
+                        for (int c = 0; c < 128; ++c)
+                            if (c < c_lo) s[c] = -INFINITY;
+                    }
+                }
+                if constexpr (kAlibi) {
+                    const float dist0 = static_cast<float>(qpos - kbase);
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            const int col = c * 32 + g * 8 + q * 2;
-                            float2 x = make_float2(s[col], s[col + 1]);
-                            x = __ffma2_rn(x, scale22, neg_m2);
-                            float2 p;
-                            if ((kPolyMask >> ((g & 1) * 4 + q)) & 1u) {
-                                p = poly_exp2_pair(x);
-                                if constexpr (kGuard) {
-                                    if (s[col] == -INFINITY) p.x = 0.0f;
-                                    if (s[col + 1] == -INFINITY) p.y = 0.0f;
-                                }
-                            } else {
-                                p.x = fast_exp2(x.x);
-                                p.y = fast_exp2(x.y);
-                            }
-                            acc[q] = __fadd2_rn(acc[q], p);
-                            pr[g * 4 + q] = pack2<kBf16>(p.x, p.y);
+                    for (int c = 0; c < 128; ++c) s[c] = fmaf(-slope2, fabsf(dist0 - static_cast<float>(c)), s[c] * scale2);
+                }
+                // tile max in log2 units; without ALiBi it is taken over the raw scores and the scale folded into the exponent's FMA
+                float m_tile;
+                {
+                    float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                    for (int c = 4; c < 128; c += 8) {
+                        mx[0] = max3(mx[0], s[c], s[c + 1]);
+                        mx[1] = max3(mx[1], s[c + 2], s[c + 3]);
+                        if (c + 4 < 128) {
+                            mx[2] = max3(mx[2], s[c + 4], s[c + 5]);
+                            mx[3] = max3(mx[3], s[c + 6], s[c + 7]);
                         }
                     }
-                    tmem_st16(tmem_s + lane_base + c * 16, pr);
-                    if (c == (kSplitSteps * 16) / 32 - 1) {
-                        // the first kSplitSteps*16 columns are stored: let the MMA warp start P V on them
-                        tmem_wait_st();
-                        tc_fence_before_sync();
-                        named_arrive(1 + 2 * qi);
+                    m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                    if constexpr (!kAlibi) m_tile *= scale2;
+                }
+                // lazy rescale: keep the old reference max unless the new one is much larger
+                float m_new = m_ref, factor = 1.0f;
+                if (m_tile > m_ref + kRescaleThreshold || m_ref == -INFINITY) {
+                    m_new = fmaxf(m_ref, m_tile);
+                    factor = (m_ref == -INFINITY) ? 0.0f : fast_exp2(m_ref - m_new);
+                }
+                const bool rescale = (j > 0) && (m_new != m_ref);
+                if (__any_sync(0xffffffffu, rescale)) {
+                    // P V of the previous tile has completed (its commit precedes s_full), so O is stable.  A row that has seen no key yet
+                    // starts from zero, whatever the values of keys that it does not see have left.
+                    const float f = rescale ? factor : 1.0f;
+                    const uint32_t seen = rescale && m_ref == -INFINITY ? 0u : 0xffffffffu;
+#pragma unroll
+                    for (int c = 0; c < D / 32; ++c) {
+                        uint32_t orow[32];
+                        tmem_ld32(tmem_o + lane_base + c * 32, orow);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) orow[i] = __float_as_uint(__uint_as_float(orow[i] & seen) * f);
+                        tmem_st32(tmem_o + lane_base + c * 32, orow);
                     }
                 }
-            };
-            if (tile_masked) exp_tile(std::true_type{});
-            else exp_tile(std::false_type{});
-            l_sum += (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y) + (acc[2].x + acc[2].y) + (acc[3].x + acc[3].y);
-            tmem_wait_st();
-            tc_fence_before_sync();
-            named_arrive(2 + 2 * qi);
-        }
+                l_sum *= (m_new != m_ref) ? factor : 1.0f;
+                m_ref = m_new;
+                const float neg_m = (m_ref == -INFINITY) ? 0.0f : -m_ref;
 
-        // ---- epilogue: rows of any place, sixteen at a time through this warp's part of the query tile's Q buffer --------------------
-        bool have_o = false;
-        if (n_tiles > 0 && fail == 0) {
-            if (mbar_wait_warp(my_o_full, 0, abort_flag)) { tc_fence_after_sync(); have_o = true; }
-            else fail = 9;
-        }
-        if (!have_o && n_union > 0) (void)mbar_wait_warp(bar_q_full, 0, abort_flag);  // (Q has landed where the rows are staged)
-        const bool gave_up = *abort_flag != 0;
-        if (gave_up) {  // (copies in flight land first)
-            const long long t0 = clock64();
-            while (clock64() - t0 < 200000) { }
-        }
-        // A wait gave up, or a visible page was not there: none of the rows may pass for a softmax.
-        if (gave_up || *bad_page != 0) l_sum = __int_as_float(0x7fc00000);
-        const bool split = w.parts > 1;
-        const long long part_row0 = static_cast<long long>(w.slot + w.part) * a.plan.rows + qi * tile_rows;
-        const float inv = split ? 1.0f : l_sum == 0.0f ? 0.0f : 1.0f / l_sum;  // (NaN stays)
-        // (a row without keys is 0, whatever the values of keys that it does not see have left)
-        auto scaled = [&](uint32_t x) { return l_sum == 0.0f ? 0u : __float_as_uint(__uint_as_float(x) * inv); };
-        if (mine) {
-            if (split) a.ml_partial[part_row0 + r] = make_float2(m_ref, l_sum);
-            else if (a.lse != nullptr)
-                a.lse[static_cast<long long>(w.first + tok) * a.heads + head] = l_sum == 0.0f ? -INFINITY : fmaf(m_ref, kLn2, logf(l_sum));
-        }
-        const uint32_t rows16 = sQ + qi * C::kTileBytes + (warp & 3) * (32 * D * 2);
-#pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-            const int first = (warp & 3) * 32 + h * 16;  // row of the tile
-            const int n_rows = min(16, min(tile_rows, (w.n - token0 - qi * tile_tokens) * a.plan.group) - first);
-            if (n_rows <= 0) break;
-#pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-                uint32_t orow[32];
-                if (have_o) {
-                    tmem_ld32(tmem_o + lane_base + c * 32, orow);
-                    tmem_wait_ld();
-                } else {
+                // P = exp2(s * scale - m), rounded to the inputs' type for the tensor core; its sum is not
+                float2 acc[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
+                const float2 neg_m2 = make_float2(neg_m, neg_m);
+                const float2 scale22 = kAlibi ? make_float2(1.0f, 1.0f) : make_float2(scale2, scale2);
+                auto exp_tile = [&](auto guard_tag) {
+                    constexpr bool kGuard = decltype(guard_tag)::value;  // the tile has masked (-inf) scores, for which the polynomial gives 2^-126
+                    constexpr uint32_t kPolyMask = poly_mask(D, kAlibi);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) orow[i] = 0u;
-                }
-                if ((lane >> 4) == h) {
+                    for (int c = 0; c < 4; ++c) {  // quarters of 32 columns
+                        uint32_t pr[16];
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        const uint32_t chunk = static_cast<uint32_t>((c * 32 + i) >> 2) ^ static_cast<uint32_t>(lane & 7);
-                        st_shared_v4(rows16 + (lane & 15) * (D * 4) + chunk * 16, scaled(orow[i]), scaled(orow[i + 1]), scaled(orow[i + 2]), scaled(orow[i + 3]));
+                        for (int g = 0; g < 4; ++g) {
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) {
+                                const int col = c * 32 + g * 8 + q * 2;
+                                float2 x = make_float2(s[col], s[col + 1]);
+                                x = __ffma2_rn(x, scale22, neg_m2);
+                                float2 p;
+                                if ((kPolyMask >> ((g & 1) * 4 + q)) & 1u) {
+                                    p = poly_exp2_pair(x);
+                                    if constexpr (kGuard) {
+                                        if (s[col] == -INFINITY) p.x = 0.0f;
+                                        if (s[col + 1] == -INFINITY) p.y = 0.0f;
+                                    }
+                                } else {
+                                    p.x = fast_exp2(x.x);
+                                    p.y = fast_exp2(x.y);
+                                }
+                                acc[q] = __fadd2_rn(acc[q], p);
+                                pr[g * 4 + q] = pack2<kBf16>(p.x, p.y);
+                            }
+                        }
+                        tmem_st16(tmem_s + lane_base + c * 16, pr);
+                        if (c == (kSplitSteps * 16) / 32 - 1) {
+                            // the first kSplitSteps*16 columns are stored: let the MMA warp start P V on them
+                            tmem_wait_st();
+                            tc_fence_before_sync();
+                            named_arrive(1 + 2 * qi);
+                        }
                     }
+                };
+                if (tile_masked) exp_tile(std::true_type{});
+                else exp_tile(std::false_type{});
+                l_sum += (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y) + (acc[2].x + acc[2].y) + (acc[3].x + acc[3].y);
+                tmem_wait_st();
+                tc_fence_before_sync();
+                named_arrive(2 + 2 * qi);
+            }
+
+            s_phase += n_tiles;
+            // ---- epilogue: rows of any place, a few at a time through this warp's room in shared memory --------------------------------
+            bool have_o = false;
+            if (n_tiles > 0) {
+                if (fail == 0 && mbar_wait_warp(my_o_full, o_phase, abort_flag)) { tc_fence_after_sync(); have_o = true; }
+                else if (fail == 0) fail = 9;
+                o_phase ^= 1;
+            }
+            // A wait gave up, or a visible page was not there: none of the rows may pass for a softmax.
+            if (g.n_tiles > 0 && (*abort_flag != 0 || bad_seg[at] != 0)) l_sum = __int_as_float(0x7fc00000);
+            const bool split = g.parts > 1;
+            const long long first_row = static_cast<long long>(g.first) + token0 + qi * tile_tokens;  // (of Q)
+            const long long part_row0 = (static_cast<long long>(g.slot) + g.part) * a.plan.rows + qi * tile_rows;
+            const float inv = split ? 1.0f : l_sum == 0.0f ? 0.0f : 1.0f / l_sum;  // (NaN stays)
+            // (a row without keys is 0, whatever the values of keys that it does not see have left)
+            auto scaled = [&](uint32_t x) { return l_sum == 0.0f ? 0u : __float_as_uint(__uint_as_float(x) * inv); };
+            if (mine) {
+                if (split) a.ml_partial[part_row0 + r] = make_float2(m_ref, l_sum);
+                else if (a.lse != nullptr) a.lse[(first_row + r_tok) * a.heads + head] = l_sum == 0.0f ? -INFINITY : fmaf(m_ref, kLn2, logf(l_sum));
+            }
+            const int rows_left = min(tile_rows, g.n_rows - qi * tile_rows) - (warp & 3) * 32;  // of this warp's 32
+            constexpr int kCols = C::kStageCols, kLanes = kCols / 4, kPerWarp = 32 / kLanes;
+            const uint32_t rows = smem_base + C::kSmemRows + warp * (32 * kCols * 4);
+            const int chunk = lane % kLanes, head0 = g.head * a.plan.group;
+#pragma unroll 1
+            for (int c = 0; c < D; c += kCols) {
+                uint32_t orow[kCols];
+#pragma unroll
+                for (int i = 0; i < kCols; ++i) orow[i] = 0u;
+                if (have_o) {
+                    if constexpr (kCols == 32) tmem_ld32(tmem_o + lane_base + c, orow);
+                    else tmem_ld16(tmem_o + lane_base + c, orow);
+                    tmem_wait_ld();
+                }
+#pragma unroll
+                for (int i = 0; i < kCols; i += 4)
+                    st_shared_v4(rows + lane * (kCols * 4) + ((i >> 2) ^ (lane & (kLanes - 1))) * 16, scaled(orow[i]), scaled(orow[i + 1]), scaled(orow[i + 2]),
+                                 scaled(orow[i + 3]));
+                __syncwarp();
+#pragma unroll 4
+                for (int k = lane / kLanes; k < 32; k += kPerWarp) {
+                    if (k >= rows_left || c + chunk * 4 >= a.head_dim) continue;
+                    const float4 o = ld_shared_f32x4(rows + k * (kCols * 4) + (chunk ^ (k & (kLanes - 1))) * 16);
+                    const int row = (warp & 3) * 32 + k;
+                    if (split) {
+                        *reinterpret_cast<float4*>(a.o_partial + (part_row0 + row) * D + c + chunk * 4) = o;
+                        continue;
+                    }
+                    const int k_tok = static_cast<int>(fast_div(a.div_group, static_cast<uint32_t>(row)));
+                    const long long to = (first_row + k_tok) * a.o_stride[0] + (head0 + row - k_tok * a.plan.group) * a.o_stride[1] + c + chunk * 4;
+                    if (a.o_is_fp32) *reinterpret_cast<float4*>(static_cast<float*>(a.o) + to) = o;
+                    else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + to) = make_uint2(pack2<kBf16>(o.x, o.y), pack2<kBf16>(o.z, o.w));
                 }
                 __syncwarp();
             }
-            constexpr int kLanes = D / 4, kPerWarp = 32 / kLanes;
-            const int chunk = lane % kLanes;
-#pragma unroll 4
-            for (int k = lane / kLanes; k < 16; k += kPerWarp) {
-                if (k >= n_rows || chunk * 4 >= a.head_dim) continue;
-                const float4 o = ld_shared_f32x4(rows16 + k * (D * 4) + static_cast<uint32_t>(chunk ^ (k & 7)) * 16);
-                if (split) {
-                    *reinterpret_cast<float4*>(a.o_partial + (part_row0 + first + k) * D + chunk * 4) = o;
-                    continue;
-                }
-                const int k_tok = static_cast<int>(fast_div(a.div_group, static_cast<uint32_t>(first + k)));
-                const long long at = (w.first + token0 + qi * tile_tokens + k_tok) * a.o_stride[0] +
-                                     (w.head * a.plan.group + first + k - k_tok * a.plan.group) * a.o_stride[1] + chunk * 4;
-                if (a.o_is_fp32) *reinterpret_cast<float4*>(static_cast<float*>(a.o) + at) = o;
-                else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + at) = make_uint2(pack2<kBf16>(o.x, o.y), pack2<kBf16>(o.z, o.w));
-            }
+            if (split && last_to_come<NQ * 128>(a, g.slot, g.parts, last_flag))
+                merge_parts<D, kBf16, NQ * 4, 8>(a, g.slot, g.parts, g.head, g.first, g.row0, g.n_rows, warp);
             __syncwarp();
+            if (lane == 0) mbar_arrive(bar_seg_free + 8 * at);
         }
-        if (split && last_to_come<NQ * 128>(a, w.slot, w.parts, reinterpret_cast<volatile int*>(smem_gen + C::kSmemMisc + 12)))
-            merge_parts<D, kBf16, NQ * 4, 4>(a, w.slot, w.parts, w.head, w.first, token0 * a.plan.group, min(a.plan.rows, (w.n - token0) * a.plan.group), warp);
     }
 
     if (fail != 0) {
@@ -548,7 +599,7 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     }
     tc_fence_before_sync();
     __syncthreads();
-    if (warp == C::kMmaWarp && n_union > 0) {
+    if (warp == C::kMmaWarp) {
         __syncwarp();
         tc_fence_after_sync();
         tmem_dealloc(tmem_base, C::kTmemCols);

@@ -99,9 +99,12 @@ struct PartLine {
         if (batch <= 32 && per <= p.one_wave) {
             auto ctas_with = [&](int y) { return __reduce_add_sync(0xffffffffu, static_cast<unsigned>(x.x * p.heads_k * parts_of(p, x.y, y))); };
             if (static_cast<long long>(ctas_with(0x3fffffff)) <= p.slots) {  // the smallest share with which all parts run at once
-                passes = 1;
-                share = max(static_cast<int>(per), p.min_share);
-                while (static_cast<long long>(ctas_with(share)) > p.slots) share += (share >> 3) + 1;  // (ends: with a part an item they fit)
+                int one = max(static_cast<int>(per), p.min_share);
+                while (static_cast<long long>(ctas_with(one)) > p.slots) one += (one >> 3) + 1;  // (ends: with a part an item they fit)
+                if (one <= max(static_cast<int>(per + (per >> 2)), 4 * p.min_share)) {  // (else a few long parts would be waited for)
+                    share = one;
+                    passes = 1;
+                }
             }
         }
         b0 = 0;
@@ -139,7 +142,8 @@ struct PartLine {
         g->slot -= g->part;
         const int blocks = __shfl_sync(0xffffffffu, x.x, src);
         g->head = static_cast<int>(static_cast<unsigned>(item) / static_cast<unsigned>(blocks));
-        g->row0 = (item - g->head * blocks) * p.rows;
+        const int blk = item - g->head * blocks;
+        g->row0 = (p.is_causal ? blocks - 1 - blk : blk) * p.rows;  // (the longest first)
         g->n_rows = min(p.rows, g->n * p.group - g->row0);
         const int p_first = g->keys - g->n;
         const int tok_lo = static_cast<int>(fast_div(div_group, static_cast<uint32_t>(g->row0)));

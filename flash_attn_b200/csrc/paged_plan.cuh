@@ -19,6 +19,7 @@ struct PagedPlan {
     int heads_k, group;
     int rows;             // rows of a block
     int block_tokens;     // tokens that a block may reach into
+    int rows_over, rows_upto;  // sequences of more rows than the one and no more than the other are this launch's
     FastDiv div_rows;
     int is_causal, window_left, window_right;
     int slots;            // CTAs that the device runs at once
@@ -26,6 +27,7 @@ struct PagedPlan {
     int long_share;       // of launches of more than one wave: parts are no shorter than this
     int waves;            // and shares no shorter than this part of a slot's tiles
     int one_wave;         // decode kernel: tiles a slot up to which all parts are to run at once
+    int most_parts;       // of an item: as many as the table's width gives (a length may be beyond it)
     int partials;         // parts of split items that there is room for (0: nothing is split)
 };
 
@@ -55,6 +57,7 @@ __device__ __forceinline__ int2 blocks_and_tiles(const PagedPlan& p, const SeqSp
     const int n = s.end - s.first;
     if (n <= 0) return make_int2(0, 0);
     const unsigned rows = static_cast<unsigned>(n) * static_cast<unsigned>(p.group);  // (tokens * heads < 2^30)
+    if (static_cast<int>(rows) <= p.rows_over || static_cast<int>(rows) > p.rows_upto) return make_int2(0, 0);
     const int blocks = static_cast<int>(fast_div(p.div_rows, rows + p.rows - 1));
     int lo, hi;
     visible_keys(p, s.keys, s.keys - n, s.keys - 1, &lo, &hi);
@@ -85,7 +88,8 @@ struct PlanScratch {
 };
 
 __device__ __forceinline__ int parts_of(const PagedPlan& p, int tiles, int share) {
-    return p.partials > 0 && tiles > share ? static_cast<int>(static_cast<unsigned>(tiles + share - 1) / static_cast<unsigned>(share)) : 1;
+    if (p.partials == 0 || tiles <= share) return 1;
+    return min(static_cast<int>(static_cast<unsigned>(tiles + share - 1) / static_cast<unsigned>(share)), p.most_parts);
 }
 __device__ __forceinline__ long long ceil_div(unsigned long long x, int d) {
     if (x <= 0xffffffffull - d) return static_cast<long long>((static_cast<unsigned>(x) + d - 1) / static_cast<unsigned>(d));  // (the long division takes twice as long)
