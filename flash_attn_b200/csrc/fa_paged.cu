@@ -199,6 +199,13 @@ int query_map(CUtensorMap* m, const fa_paged_fwd_params* p) {
                       {1, p->q_stride[1], p->q_stride[1] * group, p->q_stride[0]}, {64, group, 1, kTile / group}});
 }
 
+// The output: 64 columns of the rows of a warp.
+int output_map(CUtensorMap* m, const fa_paged_fwd_params* p) {
+    const int group = p->heads / p->cache.heads;
+    return map_of(m, {p->o, p->cache.dtype, 4, {p->cache.head_dim, group, p->cache.heads, p->tokens},
+                      {1, p->o_stride[1], p->o_stride[1] * group, p->o_stride[0]}, {64, group, 1, 32 / group}});
+}
+
 }  // namespace
 
 }  // namespace fa
@@ -251,10 +258,13 @@ int fa_paged_fwd(const fa_paged_fwd_params* p) {
     a.scale_log2 = p->softmax_scale * 1.4426950408889634f;
     a.alibi_slopes = p->alibi_slopes;
     a.o_is_fp32 = p->o_dtype == FA_DTYPE_FP32;
+    a.o_units = (p->tokens == 1 || p->o_stride[0] % 8 == 0) && (p->heads == 1 || p->o_stride[1] % 8 == 0);
+    a.o_tma = a.o_units && !a.o_is_fp32 && 32 % a.plan.group == 0 && p->o_stride[0] < (1LL << 39) && p->o_stride[1] * a.plan.group < (1LL << 39) &&
+              p->o_stride[0] >= 0 && p->o_stride[1] >= 0;
     a.status = p->status;
     cudaStream_t stream = static_cast<cudaStream_t>(p->stream);
     const bool bf16 = c.dtype == FA_DTYPE_BF16;
-    CUtensorMap tq, tk, tv;
+    CUtensorMap tq, tk, tv, to = {};
     if ((rc = page_maps(&tk, &tv, c, &a)) != FA_OK) return rc;
     cudaError_t e = cudaSuccess;
     for (int i = 0; i < all.n && e == cudaSuccess; ++i) {
@@ -283,8 +293,9 @@ int fa_paged_fwd(const fa_paged_fwd_params* p) {
             continue;
         }
         if ((rc = query_map(&tq, p)) != FA_OK) return rc;
-        if (l.wide == 64) e = l.query_tiles == 1 ? launch_paged_tiled<64, 1>(a, tq, tk, tv, bf16, grid, stream) : launch_paged_tiled<64, 2>(a, tq, tk, tv, bf16, grid, stream);
-        else e = l.query_tiles == 1 ? launch_paged_tiled<128, 1>(a, tq, tk, tv, bf16, grid, stream) : launch_paged_tiled<128, 2>(a, tq, tk, tv, bf16, grid, stream);
+        if (a.o_tma && (rc = output_map(&to, p)) != FA_OK) return rc;
+        if (l.wide == 64) e = l.query_tiles == 1 ? launch_paged_tiled<64, 1>(a, tq, tk, tv, to, bf16, grid, stream) : launch_paged_tiled<64, 2>(a, tq, tk, tv, to, bf16, grid, stream);
+        else e = l.query_tiles == 1 ? launch_paged_tiled<128, 1>(a, tq, tk, tv, to, bf16, grid, stream) : launch_paged_tiled<128, 2>(a, tq, tk, tv, to, bf16, grid, stream);
     }
     return e == cudaSuccess ? FA_OK : FA_ERR_CUDA;
 }

@@ -95,9 +95,9 @@ struct TCfg {
     static constexpr int kSmemQ = 0;
     static constexpr int kSmemK = NQ * kTileBytes;
     static constexpr int kSmemV = kSmemK + kStages * kTileBytes;
-    static constexpr int kStageCols = NQ == 2 ? 32 : 16;               // columns of its output rows that a warp has in shared memory at once
+    static constexpr int kStageBytes = NQ == 2 || D == 64 ? 4096 : 2048;          // of its output rows that a warp has in shared memory at once
     static constexpr int kSmemRows = kSmemV + kStages * kTileBytes;
-    static constexpr int kSmemBar = kSmemRows + NQ * 4 * 32 * kStageCols * 4;
+    static constexpr int kSmemBar = kSmemRows + NQ * 4 * kStageBytes;
     static constexpr int kNumBars = 2 + 2 * NQ + 4 * kStages + 2 * kSegs + 1;
     static constexpr int kSmemMisc = (kSmemBar + 8 * kNumBars + 15) / 16 * 16;  // tensor-memory address, abort flag, last part's flag
     static constexpr int kSmemSegs = kSmemMisc + 16 + 4 * kSegs;                // (which parts met a bad page;) PagedSeg[kSegs], a taken CTA
@@ -108,7 +108,7 @@ struct TCfg {
 template <int D, int NQ, bool kBf16, bool kAlibi>
 __global__ void __launch_bounds__(TCfg<D, NQ>::kThreads, NQ == 1 ? 2 : 1)
 paged_tiled_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
-                   const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ PagedArgs a) {
+                   const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_o, const __grid_constant__ PagedArgs a) {
     using C = TCfg<D, NQ>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -543,52 +543,115 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             const long long first_row = static_cast<long long>(g.first) + token0 + qi * tile_tokens;  // (of Q)
             const long long part_row0 = (static_cast<long long>(g.slot) + g.part) * a.plan.rows + qi * tile_rows;
             const float inv = split ? 1.0f : l_sum == 0.0f ? 0.0f : 1.0f / l_sum;  // (NaN stays)
-            // (a row without keys is 0, whatever the values of keys that it does not see have left)
-            auto scaled = [&](uint32_t x) { return l_sum == 0.0f ? 0u : __float_as_uint(__uint_as_float(x) * inv); };
             if (mine) {
                 if (split) a.ml_partial[part_row0 + r] = make_float2(m_ref, l_sum);
                 else if (a.lse != nullptr) a.lse[(first_row + r_tok) * a.heads + head] = l_sum == 0.0f ? -INFINITY : fmaf(m_ref, kLn2, logf(l_sum));
             }
             const int rows_left = min(tile_rows, g.n_rows - qi * tile_rows) - (warp & 3) * 32;  // of this warp's 32
-            constexpr int kCols = C::kStageCols, kLanes = kCols / 4, kPerWarp = 32 / kLanes;
-            const uint32_t rows = smem_base + C::kSmemRows + warp * (32 * kCols * 4);
-            const int chunk = lane % kLanes, head0 = g.head * a.plan.group;
+            float o[D];
+#pragma unroll
+            for (int c = 0; c < D; c += 32) {
+                uint32_t orow[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) orow[i] = 0u;
+                if (have_o) tmem_ld32(tmem_o + lane_base + c, orow);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[c + i] = __uint_as_float(orow[i]);
+            }
+            if (have_o) tmem_wait_ld();
+            if (__any_sync(0xffffffffu, l_sum == 0.0f)) {  // (a row without keys is 0, whatever the values of keys that it does not see have left)
+#pragma unroll
+                for (int c = 0; c < D; ++c) o[c] = l_sum == 0.0f ? 0.0f : o[c];
+            }
+#pragma unroll
+            for (int c = 0; c < D; ++c) o[c] *= inv;
+            const uint32_t rows = smem_base + C::kSmemRows + warp * C::kStageBytes;
+            if (lane == 0) tma_store_wait_read();  // (what the part before has left there)
+            __syncwarp();
+            // kRows rows of the warp in turn: laid out in shared memory by their threads, 16-byte units swizzled over eight rows, and
+            // written by the whole warp, 16 bytes a lane.
+            const int head0 = g.head * a.plan.group;
+            auto place = [&](int k) -> long long {  // element of row k of the warp in the output
+                const int row = (warp & 3) * 32 + k, k_tok = static_cast<int>(fast_div(a.div_group, static_cast<uint32_t>(row)));
+                return (first_row + k_tok) * a.o_stride[0] + (head0 + row - k_tok * a.plan.group) * a.o_stride[1];
+            };
+            if (split || a.o_is_fp32) {
+                constexpr int kRows = C::kStageBytes / (D * 4), kUnits = D / 4, kPerWarp = 32 / kUnits;
 #pragma unroll 1
-            for (int c = 0; c < D; c += kCols) {
-                uint32_t orow[kCols];
+                for (int h = 0; h < 32; h += kRows) {
+                    if (lane / kRows == h / kRows) {
 #pragma unroll
-                for (int i = 0; i < kCols; ++i) orow[i] = 0u;
-                if (have_o) {
-                    if constexpr (kCols == 32) tmem_ld32(tmem_o + lane_base + c, orow);
-                    else tmem_ld16(tmem_o + lane_base + c, orow);
-                    tmem_wait_ld();
-                }
-#pragma unroll
-                for (int i = 0; i < kCols; i += 4)
-                    st_shared_v4(rows + lane * (kCols * 4) + ((i >> 2) ^ (lane & (kLanes - 1))) * 16, scaled(orow[i]), scaled(orow[i + 1]), scaled(orow[i + 2]),
-                                 scaled(orow[i + 3]));
-                __syncwarp();
-#pragma unroll 4
-                for (int k = lane / kLanes; k < 32; k += kPerWarp) {
-                    if (k >= rows_left || c + chunk * 4 >= a.head_dim) continue;
-                    const float4 o = ld_shared_f32x4(rows + k * (kCols * 4) + (chunk ^ (k & (kLanes - 1))) * 16);
-                    const int row = (warp & 3) * 32 + k;
-                    if (split) {
-                        *reinterpret_cast<float4*>(a.o_partial + (part_row0 + row) * D + c + chunk * 4) = o;
-                        continue;
+                        for (int i = 0; i < kUnits; ++i)
+                            st_shared_v4(rows + (lane % kRows) * (D * 4) + (i ^ (lane & 7)) * 16, __float_as_uint(o[4 * i]), __float_as_uint(o[4 * i + 1]),
+                                         __float_as_uint(o[4 * i + 2]), __float_as_uint(o[4 * i + 3]));
                     }
-                    const int k_tok = static_cast<int>(fast_div(a.div_group, static_cast<uint32_t>(row)));
-                    const long long to = (first_row + k_tok) * a.o_stride[0] + (head0 + row - k_tok * a.plan.group) * a.o_stride[1] + c + chunk * 4;
-                    if (a.o_is_fp32) *reinterpret_cast<float4*>(static_cast<float*>(a.o) + to) = o;
-                    else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + to) = make_uint2(pack2<kBf16>(o.x, o.y), pack2<kBf16>(o.z, o.w));
+                    __syncwarp();
+#pragma unroll
+                    for (int k0 = 0; k0 < kRows; k0 += kPerWarp) {
+                        const int k = h + k0 + lane / kUnits, u = lane % kUnits;
+                        if (k >= rows_left || u * 4 >= a.head_dim) continue;
+                        const float4 v = ld_shared_f32x4(rows + (k % kRows) * (D * 4) + (u ^ (k & 7)) * 16);
+                        float* to = split ? a.o_partial + (part_row0 + (warp & 3) * 32 + k) * D : static_cast<float*>(a.o) + place(k);
+                        *reinterpret_cast<float4*>(to + u * 4) = v;
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
+            } else {
+                constexpr int kRows = C::kStageBytes / (D * 2), kUnits = D / 8, kPerWarp = 32 / kUnits;
+                uint32_t packed[D / 2];
+#pragma unroll
+                for (int c = 0; c < D / 2; ++c) packed[c] = pack2<kBf16>(o[2 * c], o[2 * c + 1]);
+                const bool whole = C::kStageBytes == 4096 && a.o_tma && rows_left >= 32;
+                if (whole) {  // all 32 rows of the warp: by TMA, 64 columns at a time (4.3 us of a part by hand, ZZ so)
+#pragma unroll
+                    for (int half = 0; half < D / 64; ++half) {
+                        if (half > 0) {
+                            if (lane == 0) tma_store_wait_read();
+                            __syncwarp();
+                        }
+#pragma unroll
+                        for (int u = 0; u < 8; ++u)
+                            st_shared_v4(rows + lane * 128 + ((u ^ (lane & 7)) << 4), packed[half * 32 + 4 * u], packed[half * 32 + 4 * u + 1],
+                                         packed[half * 32 + 4 * u + 2], packed[half * 32 + 4 * u + 3]);
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) {
+                            tma_store_4d(&tmap_o, rows, half * 64, 0, g.head,
+                                         static_cast<int>(first_row) + static_cast<int>(fast_div(a.div_group, static_cast<uint32_t>((warp & 3) * 32))));
+                            tma_store_commit();
+                        }
+                    }
+                }
+#pragma unroll 1
+                for (int h = whole ? 32 : 0; h < 32; h += kRows) {
+                    if (lane / kRows == h / kRows) {
+#pragma unroll
+                        for (int i = 0; i < kUnits; ++i)
+                            st_shared_v4(rows + (lane % kRows) * (D * 2) + (i ^ (lane & 7)) * 16, packed[4 * i], packed[4 * i + 1], packed[4 * i + 2], packed[4 * i + 3]);
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int k0 = 0; k0 < kRows; k0 += kPerWarp) {
+                        const int k = h + k0 + lane / kUnits, u = lane % kUnits;
+                        if (k >= rows_left || u * 8 >= a.head_dim) continue;
+                        const float4 v = ld_shared_f32x4(rows + (k % kRows) * (D * 2) + (u ^ (k & 7)) * 16);
+                        uint16_t* to = static_cast<uint16_t*>(a.o) + place(k) + u * 8;
+                        if (a.o_units) {
+                            *reinterpret_cast<float4*>(to) = v;
+                        } else {
+                            *reinterpret_cast<float2*>(to) = make_float2(v.x, v.y);
+                            *reinterpret_cast<float2*>(to + 4) = make_float2(v.z, v.w);
+                        }
+                    }
+                    __syncwarp();
+                }
             }
             if (split && last_to_come<NQ * 128>(a, g.slot, g.parts, last_flag))
                 merge_parts<D, kBf16, NQ * 4, 8>(a, g.slot, g.parts, g.head, g.first, g.row0, g.n_rows, warp);
             __syncwarp();
             if (lane == 0) mbar_arrive(bar_seg_free + 8 * at);
         }
+        if (lane == 0) tma_store_wait_read();
     }
 
     if (fail != 0) {
@@ -609,7 +672,7 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
 }  // namespace
 
 template <>
-cudaError_t launch_paged_tiled<FA_PAGED_D, FA_PAGED_NQ>(const PagedArgs& a, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, bool bf16,
+cudaError_t launch_paged_tiled<FA_PAGED_D, FA_PAGED_NQ>(const PagedArgs& a, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& to, bool bf16,
                                                         unsigned grid, cudaStream_t stream) {
     using C = TCfg<FA_PAGED_D, FA_PAGED_NQ>;
     int dev = 0;
@@ -632,7 +695,7 @@ cudaError_t launch_paged_tiled<FA_PAGED_D, FA_PAGED_NQ>(const PagedArgs& a, cons
             if (err != cudaSuccess) return err;
             if (dev >= 0 && dev < 64) done[dev].store(true, std::memory_order_release);
         }
-        return cudaLaunchKernelEx(&cfg, kern, tq, tk, tv, a);
+        return cudaLaunchKernelEx(&cfg, kern, tq, tk, tv, to, a);
     };
     if (a.alibi_slopes != nullptr)
         return bf16 ? run(paged_tiled_kernel<FA_PAGED_D, FA_PAGED_NQ, true, true>, configured[0])

@@ -36,6 +36,8 @@ struct PagedArgs {
     float scale_log2;
     const float* alibi_slopes;
     int o_is_fp32;
+    int o_units;              // rows of the output begin at 16 bytes
+    int o_tma;                // and 32 rows of a K/V head are whole tokens: they have a tensor map
     float* o_partial;         // [parts of split items][plan.rows][64 or 128], un-normalised
     float2* ml_partial;       // [parts of split items][plan.rows]: maximum (log2 units) and sum
     unsigned long long* counts;  // [parts of split items]: those of an item's first part are its count
@@ -47,12 +49,12 @@ cudaError_t launch_paged_decode(const PagedArgs& a, const CUtensorMap& tk, const
                                 cudaStream_t stream);
 // D = 64 or 128 (head_dim rounded up), NQ query tiles a block.
 template <int D, int NQ>
-cudaError_t launch_paged_tiled(const PagedArgs& a, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, bool bf16, unsigned grid,
-                               cudaStream_t stream);
-template <> cudaError_t launch_paged_tiled<64, 1>(const PagedArgs&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, bool, unsigned, cudaStream_t);
-template <> cudaError_t launch_paged_tiled<64, 2>(const PagedArgs&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, bool, unsigned, cudaStream_t);
-template <> cudaError_t launch_paged_tiled<128, 1>(const PagedArgs&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, bool, unsigned, cudaStream_t);
-template <> cudaError_t launch_paged_tiled<128, 2>(const PagedArgs&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, bool, unsigned, cudaStream_t);
+cudaError_t launch_paged_tiled(const PagedArgs& a, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& to, bool bf16,
+                               unsigned grid, cudaStream_t stream);
+template <> cudaError_t launch_paged_tiled<64, 1>(const PagedArgs&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, bool, unsigned, cudaStream_t);
+template <> cudaError_t launch_paged_tiled<64, 2>(const PagedArgs&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, bool, unsigned, cudaStream_t);
+template <> cudaError_t launch_paged_tiled<128, 1>(const PagedArgs&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, bool, unsigned, cudaStream_t);
+template <> cudaError_t launch_paged_tiled<128, 2>(const PagedArgs&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, bool, unsigned, cudaStream_t);
 
 #ifdef __CUDACC__
 // The pages of a tile of 128 keys, as the lanes of the warp that loads them have them: a box a lane.
