@@ -17,7 +17,7 @@ namespace {
 
 // A part is not worth starting for fewer tiles than min_share; launches of more than one wave are cut into `waves` of parts, which are no
 // shorter than long_share.
-constexpr int kMinShare = 4, kLongShare = 24, kPagedWaves = 3;
+constexpr int kMinShare = 8, kLongShare = 16, kPagedWaves = 3;
 // The decode kernel's: a megabyte of K and V at least (kDecodeLongShare tiles of 128 columns; 64 sequences of 100 .. 8192 keys, 8 K/V
 // heads of 128 columns: 82 us, with 8 tiles 84, with 24 tiles 88; 24 sequences of 500 .. 4000 keys, 16 heads of 64 columns: 49 us with
 // 32 tiles, 54 with 16), and the tiles a CTA up to which a launch is one wave (4 sequences of 98304 .. 131072 keys: 298 us, in waves 309).

@@ -539,15 +539,6 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             }
             // A wait gave up, or a visible page was not there: none of the rows may pass for a softmax.
             if (g.n_tiles > 0 && (*abort_flag != 0 || bad_seg[at] != 0)) l_sum = __int_as_float(0x7fc00000);
-            const bool split = g.parts > 1;
-            const long long first_row = static_cast<long long>(g.first) + token0 + qi * tile_tokens;  // (of Q)
-            const long long part_row0 = (static_cast<long long>(g.slot) + g.part) * a.plan.rows + qi * tile_rows;
-            const float inv = split ? 1.0f : l_sum == 0.0f ? 0.0f : 1.0f / l_sum;  // (NaN stays)
-            if (mine) {
-                if (split) a.ml_partial[part_row0 + r] = make_float2(m_ref, l_sum);
-                else if (a.lse != nullptr) a.lse[(first_row + r_tok) * a.heads + head] = l_sum == 0.0f ? -INFINITY : fmaf(m_ref, kLn2, logf(l_sum));
-            }
-            const int rows_left = min(tile_rows, g.n_rows - qi * tile_rows) - (warp & 3) * 32;  // of this warp's 32
             float o[D];
 #pragma unroll
             for (int c = 0; c < D; c += 32) {
@@ -559,10 +550,57 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                 for (int i = 0; i < 32; ++i) o[c + i] = __uint_as_float(orow[i]);
             }
             if (have_o) tmem_wait_ld();
+            bool last = true;
+            if (g.parts > 1) {
+                // A part's rows lie column group by column group, so that the threads, a row each, write and read side by side.
+                const long long step = a.plan.rows;
+                const long long row0 = static_cast<long long>(g.slot) * step + qi * tile_rows + r;  // part 0's
+                auto row_of = [&](int part) { return reinterpret_cast<float4*>(a.o_partial) + (g.slot + static_cast<long long>(part)) * step * (D / 4) + qi * tile_rows + r; };
+                if (mine) {
+                    float4* to = row_of(g.part);
+#pragma unroll
+                    for (int c = 0; c < D / 4; ++c) to[c * step] = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+                    a.ml_partial[row0 + g.part * step] = make_float2(m_ref, l_sum);
+                }
+                last = last_to_come<NQ * 128>(a, g.slot, g.parts, last_flag);
+                if (last) {
+                    // O = sum_j 2^(m_j - m) O_j, l = sum_j 2^(m_j - m) l_j, in the order of the parts whoever is last
+#pragma unroll
+                    for (int c = 0; c < D; ++c) o[c] = 0.0f;
+                    m_ref = -INFINITY;
+                    l_sum = 0.0f;
+                    if (mine) {
+#pragma unroll 4
+                        for (int j = 0; j < g.parts; ++j) m_ref = fmaxf(m_ref, __ldcg(a.ml_partial + row0 + j * step).x);
+                        const float base = m_ref == -INFINITY ? 0.0f : m_ref;
+#pragma unroll 1
+                        for (int j = 0; j < g.parts; ++j) {
+                            const float2 x = __ldcg(a.ml_partial + row0 + j * step);
+                            const float f = exp2f(x.x - base);
+                            l_sum += x.x == -INFINITY ? x.y : f * x.y;  // (a part that saw no key: 0; one that saw only NaN: NaN)
+                            const float4* from = row_of(j);
+                            if (f == 0.0f) continue;  // (nothing, or what masked values made of it)
+#pragma unroll
+                            for (int c = 0; c < D / 4; ++c) {
+                                const float4 v = __ldcg(from + c * step);
+                                o[4 * c] = fmaf(f, v.x, o[4 * c]);
+                                o[4 * c + 1] = fmaf(f, v.y, o[4 * c + 1]);
+                                o[4 * c + 2] = fmaf(f, v.z, o[4 * c + 2]);
+                                o[4 * c + 3] = fmaf(f, v.w, o[4 * c + 3]);
+                            }
+                        }
+                    }
+                }
+            }
+            const long long first_row = static_cast<long long>(g.first) + token0 + qi * tile_tokens;  // (of Q)
+            // of this warp's 32 (a part that others will put together: none)
+            const int rows_left = last ? min(tile_rows, g.n_rows - qi * tile_rows) - (warp & 3) * 32 : 0;
+            if (last && mine && a.lse != nullptr) a.lse[(first_row + r_tok) * a.heads + head] = l_sum == 0.0f ? -INFINITY : fmaf(m_ref, kLn2, logf(l_sum));
             if (__any_sync(0xffffffffu, l_sum == 0.0f)) {  // (a row without keys is 0, whatever the values of keys that it does not see have left)
 #pragma unroll
                 for (int c = 0; c < D; ++c) o[c] = l_sum == 0.0f ? 0.0f : o[c];
             }
+            const float inv = l_sum == 0.0f ? 0.0f : 1.0f / l_sum;  // (NaN stays)
 #pragma unroll
             for (int c = 0; c < D; ++c) o[c] *= inv;
             const uint32_t rows = smem_base + C::kSmemRows + warp * C::kStageBytes;
@@ -575,7 +613,7 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                 const int row = (warp & 3) * 32 + k, k_tok = static_cast<int>(fast_div(a.div_group, static_cast<uint32_t>(row)));
                 return (first_row + k_tok) * a.o_stride[0] + (head0 + row - k_tok * a.plan.group) * a.o_stride[1];
             };
-            if (split || a.o_is_fp32) {
+            if (rows_left > 0 && a.o_is_fp32) {
                 constexpr int kRows = C::kStageBytes / (D * 4), kUnits = D / 4, kPerWarp = 32 / kUnits;
 #pragma unroll 1
                 for (int h = 0; h < 32; h += kRows) {
@@ -591,18 +629,17 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                         const int k = h + k0 + lane / kUnits, u = lane % kUnits;
                         if (k >= rows_left || u * 4 >= a.head_dim) continue;
                         const float4 v = ld_shared_f32x4(rows + (k % kRows) * (D * 4) + (u ^ (k & 7)) * 16);
-                        float* to = split ? a.o_partial + (part_row0 + (warp & 3) * 32 + k) * D : static_cast<float*>(a.o) + place(k);
-                        *reinterpret_cast<float4*>(to + u * 4) = v;
+                        *reinterpret_cast<float4*>(static_cast<float*>(a.o) + place(k) + u * 4) = v;
                     }
                     __syncwarp();
                 }
-            } else {
+            } else if (rows_left > 0) {
                 constexpr int kRows = C::kStageBytes / (D * 2), kUnits = D / 8, kPerWarp = 32 / kUnits;
                 uint32_t packed[D / 2];
 #pragma unroll
                 for (int c = 0; c < D / 2; ++c) packed[c] = pack2<kBf16>(o[2 * c], o[2 * c + 1]);
                 const bool whole = C::kStageBytes == 4096 && a.o_tma && rows_left >= 32;
-                if (whole) {  // all 32 rows of the warp: by TMA, 64 columns at a time (4.3 us of a part by hand, ZZ so)
+                if (whole) {  // all 32 rows of the warp: by TMA, 64 columns at a time (prompts of six requests: 45.4 us, by hand 50.5)
 #pragma unroll
                     for (int half = 0; half < D / 64; ++half) {
                         if (half > 0) {
@@ -646,8 +683,6 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                     __syncwarp();
                 }
             }
-            if (split && last_to_come<NQ * 128>(a, g.slot, g.parts, last_flag))
-                merge_parts<D, kBf16, NQ * 4, 8>(a, g.slot, g.parts, g.head, g.first, g.row0, g.n_rows, warp);
             __syncwarp();
             if (lane == 0) mbar_arrive(bar_seg_free + 8 * at);
         }
