@@ -16,8 +16,8 @@ namespace fa {
 namespace {
 
 // A part is not worth starting for fewer tiles than min_share; launches of more than one wave are cut into `waves` of parts, which are no
-// shorter than long_share.
-constexpr int kMinShare = 8, kLongShare = 16, kPagedWaves = 3;
+// shorter than long_share.  (Chunks: with parts of 4 and 24 tiles at least a seventh of 14 batches takes a sixth longer, with 16 and 48 none less.)
+constexpr int kMinShare = 8, kLongShare = 16, kPagedWaves = 3, kOneWave = 24;
 // The decode kernel's: a megabyte of K and V at least (kDecodeLongShare tiles of 128 columns; 64 sequences of 100 .. 8192 keys, 8 K/V
 // heads of 128 columns: 82 us, with 8 tiles 84, with 24 tiles 88; 24 sequences of 500 .. 4000 keys, 16 heads of 64 columns: 49 us with
 // 32 tiles, 54 with 16), and the tiles a CTA up to which a launch is one wave (4 sequences of 98304 .. 131072 keys: 298 us, in waves 309).
@@ -54,7 +54,6 @@ struct PagedLaunch {
     int query_tiles;           // tiled kernel: of a block
     int rows;                  // of a block
     int slots;                 // CTAs that run at once
-    int rows_over, rows_upto;  // sequences of so many rows it takes
     int min_share, long_share, waves, most_parts;
     int wide;                  // columns of a partial row: head_dim rounded up
     long long items;           // at most so many blocks of rows there are, over all K/V heads
@@ -62,16 +61,15 @@ struct PagedLaunch {
     size_t count_bytes, ml_bytes, o_bytes, bytes;  // workspace: counts of parts, maxima and sums of partial rows, the rows, and all
 };
 
-int columns_of(long long rows) { return rows == 1 ? 1 : rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 ? 16 : 0; }
-
-// columns: of the decode kernel, 0: the tiled kernel.
-PagedLaunch plan_launch(const fa_paged_fwd_params* p, int sms, int columns) {
+// (A launch of each kernel where single tokens stand beside chunks was slower in six of eight such batches, by up to a half: what the two
+// have to set up and the end of the one are not overlapped.)
+PagedLaunch plan_launch(const fa_paged_fwd_params* p, int sms) {
     const fa_paged_kv& c = p->cache;
     PagedLaunch l = {};
     const int group = p->heads / c.heads;
     const long long rows = static_cast<long long>(std::min<int64_t>(p->max_seqlen_q, p->tokens)) * group;
     const int tile_rows = kTile / group * group;
-    l.columns = columns;
+    l.columns = rows == 1 ? 1 : rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 ? 16 : 0;
     l.query_tiles = l.columns ? 0 : rows <= tile_rows ? 1 : 2;
     l.rows = l.columns ? l.columns : l.query_tiles * tile_rows;
     l.wide = c.head_dim <= 64 ? 64 : 128;
@@ -95,31 +93,6 @@ PagedLaunch plan_launch(const fa_paged_fwd_params* p, int sms, int columns) {
     l.o_bytes = room(static_cast<size_t>(l.partials) * l.rows * l.wide * sizeof(float));
     if (l.partials > 0) l.bytes = l.count_bytes + l.ml_bytes + l.o_bytes;
     return l;
-}
-
-// The launches of a call: one, or where sequences of few rows stand beside long chunks (the mean is a quarter of the most, or less) the
-// decode kernel for the ones and the tiled kernel for the others.  32 single tokens and a chunk of 512: MIXED us, by the tiled
-// kernel alone 112; where there are no single tokens the launch that finds nothing costs EMPTY us.
-struct PagedLaunches {
-    PagedLaunch one[2];
-    int n;
-    size_t bytes;  // (they run one behind the other, in the same workspace)
-};
-PagedLaunches plan_launches(const fa_paged_fwd_params* p, int sms) {
-    const fa_paged_kv& c = p->cache;
-    const int group = p->heads / c.heads;
-    const int64_t most = std::min<int64_t>(p->max_seqlen_q, p->tokens);
-    const int columns = columns_of(most * group), few = std::max(columns_of(group), 4);
-    PagedLaunches all = {};
-    all.one[all.n++] = plan_launch(p, sms, columns);
-    if (columns == 0 && columns_of(group) != 0 && c.cu_seqlens_q && c.batch > 1 && p->tokens <= most * c.batch / 4) all.one[all.n++] = plan_launch(p, sms, few);
-    all.one[0].rows_upto = 0x7fffffff;
-    if (all.n == 2) {
-        all.one[0].rows_over = all.one[1].rows_upto = few;
-        all.bytes = all.one[1].bytes;
-    }
-    all.bytes = std::max(all.bytes, all.one[0].bytes);
-    return all;
 }
 
 // A tensor map: extents, strides (elements; of a dimension of one any will do) and box, innermost first.  The last ones are kept per
@@ -218,7 +191,7 @@ size_t fa_paged_fwd_workspace_bytes(const fa_paged_fwd_params* p) {
     if (check_fwd(p) != FA_OK) return 0;
     int sms = 148, major = 10;
     if (current_device(&sms, &major) != FA_OK) sms = 148;
-    return plan_launches(p, sms).bytes;
+    return plan_launch(p, sms).bytes;
 }
 
 int fa_paged_fwd(const fa_paged_fwd_params* p) {
@@ -227,11 +200,10 @@ int fa_paged_fwd(const fa_paged_fwd_params* p) {
     int sms = 0, major = 0;
     if ((rc = current_device(&sms, &major)) != FA_OK) return rc;
     if (major != 10) return FA_ERR_NOT_SM100;
-    const PagedLaunches all = plan_launches(p, sms);
-    for (int i = 0; i < all.n; ++i)
-        if (all.one[i].grid > 0x7fffffffLL) return FA_ERR_TOO_LARGE;
-    if (all.bytes > 0 && (!p->workspace || p->workspace_bytes < all.bytes)) return FA_ERR_WORKSPACE;
-    if (all.bytes > 0 && (reinterpret_cast<uintptr_t>(p->workspace) & 15u)) return FA_ERR_INVALID_ARG;
+    const PagedLaunch l = plan_launch(p, sms);
+    if (l.grid > 0x7fffffffLL) return FA_ERR_TOO_LARGE;
+    if (l.bytes > 0 && (!p->workspace || p->workspace_bytes < l.bytes)) return FA_ERR_WORKSPACE;
+    if (l.bytes > 0 && (reinterpret_cast<uintptr_t>(p->workspace) & 15u)) return FA_ERR_INVALID_ARG;
     const fa_paged_kv& c = p->cache;
     PagedArgs a = {};
     a.plan.seq = {c.seqlens_k, c.cu_seqlens_q, c.batch, static_cast<int>(p->tokens)};
@@ -266,32 +238,27 @@ int fa_paged_fwd(const fa_paged_fwd_params* p) {
     const bool bf16 = c.dtype == FA_DTYPE_BF16;
     CUtensorMap tq, tk, tv, to = {};
     if ((rc = page_maps(&tk, &tv, c, &a)) != FA_OK) return rc;
-    cudaError_t e = cudaSuccess;
-    for (int i = 0; i < all.n && e == cudaSuccess; ++i) {
-        const PagedLaunch& l = all.one[i];
-        a.plan.rows = l.rows;
-        a.plan.block_tokens = l.rows / a.plan.group + 2;  // (it may begin and end inside a token)
-        a.plan.rows_over = l.rows_over;
-        a.plan.rows_upto = l.rows_upto;
-        a.plan.div_rows = make_fastdiv(static_cast<uint32_t>(l.rows));
-        a.plan.slots = l.slots;
-        a.plan.min_share = l.min_share;
-        a.plan.long_share = l.long_share;
-        a.plan.waves = l.waves;
-        a.plan.most_parts = l.most_parts;
-        a.plan.one_wave = l.columns ? kDecodeOneWave : kLongShare;
-        a.plan.partials = static_cast<int>(l.partials);
-        if (l.bytes > 0) {
-            char* room = static_cast<char*>(p->workspace);
-            a.counts = reinterpret_cast<unsigned long long*>(room);
-            a.ml_partial = reinterpret_cast<float2*>(room + l.count_bytes);
-            a.o_partial = reinterpret_cast<float*>(room + l.count_bytes + l.ml_bytes);
-        }
-        const unsigned grid = static_cast<unsigned>(l.grid);
-        if (l.columns) {
-            e = launch_paged_decode(a, tk, tv, l.columns, bf16, grid, stream);
-            continue;
-        }
+    a.plan.rows = l.rows;
+    a.plan.block_tokens = l.rows / a.plan.group + 2;  // (it may begin and end inside a token)
+    a.plan.div_rows = make_fastdiv(static_cast<uint32_t>(l.rows));
+    a.plan.slots = l.slots;
+    a.plan.min_share = l.min_share;
+    a.plan.long_share = l.long_share;
+    a.plan.waves = l.waves;
+    a.plan.most_parts = l.most_parts;
+    a.plan.one_wave = l.columns ? kDecodeOneWave : kOneWave;
+    a.plan.partials = static_cast<int>(l.partials);
+    if (l.bytes > 0) {
+        char* room = static_cast<char*>(p->workspace);
+        a.counts = reinterpret_cast<unsigned long long*>(room);
+        a.ml_partial = reinterpret_cast<float2*>(room + l.count_bytes);
+        a.o_partial = reinterpret_cast<float*>(room + l.count_bytes + l.ml_bytes);
+    }
+    const unsigned grid = static_cast<unsigned>(l.grid);
+    cudaError_t e;
+    if (l.columns) {
+        e = launch_paged_decode(a, tk, tv, l.columns, bf16, grid, stream);
+    } else {
         if ((rc = query_map(&tq, p)) != FA_OK) return rc;
         if (a.o_tma && (rc = output_map(&to, p)) != FA_OK) return rc;
         if (l.wide == 64) e = l.query_tiles == 1 ? launch_paged_tiled<64, 1>(a, tq, tk, tv, to, bf16, grid, stream) : launch_paged_tiled<64, 2>(a, tq, tk, tv, to, bf16, grid, stream);

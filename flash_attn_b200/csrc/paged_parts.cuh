@@ -1,4 +1,4 @@
-// How the decode kernel over a paged cache shares a launch out.
+// How the kernels over a paged cache share a launch out.
 //
 // An item (a block of rows of a sequence and K/V head; paged_plan.cuh) is cut into equal parts of at most `share` tiles, and the parts of
 // all items are numbered.  The grid is as large as their number can be; CTA i begins with part i, and while it works on one its
