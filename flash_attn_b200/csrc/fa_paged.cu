@@ -16,7 +16,8 @@ namespace fa {
 namespace {
 
 // A part is not worth starting for fewer tiles than min_share; launches of more than one wave are cut into `waves` of parts, which are no
-// shorter than long_share.  (Chunks: with parts of 4 and 24 tiles at least a seventh of 14 batches takes a sixth longer, with 16 and 48 none less.)
+// shorter than long_share.  (Of 14 batches of chunks two took a sixth longer with
+// parts of 4 tiles and more, none less with 16 and more.)
 constexpr int kMinShare = 8, kLongShare = 16, kPagedWaves = 3, kOneWave = 24;
 // The decode kernel's: a megabyte of K and V at least (kDecodeLongShare tiles of 128 columns; 64 sequences of 100 .. 8192 keys, 8 K/V
 // heads of 128 columns: 82 us, with 8 tiles 84, with 24 tiles 88; 24 sequences of 500 .. 4000 keys, 16 heads of 64 columns: 49 us with

@@ -13,6 +13,8 @@ namespace fa {
 //     pool's tokens in eights, pages and (where their stride is a number of eights) heads together: (64, 8, 2, eights, heads).
 //   half rows: 64 columns, a box for each half: (columns, slots, heads, pages).  For 64-wide heads, heads that do not fill their
 //     columns, and strides that the other does not reach.
+// A box takes the SM about 80 cycles to issue however small it is, which is what small pages cost: 64 x 8192 keys, 8 K/V heads of 128
+// columns, pages of 16 tokens: 347 us with half rows, 322 with whole ones (309 with pages of 128).
 struct PageBoxes {
     int page_step, head_step;  // whole rows: eights from one page and one head to the next
     int head_coord;            // 1: heads have a coordinate of their own
