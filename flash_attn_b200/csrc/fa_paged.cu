@@ -1,15 +1,10 @@
 // Attention of new tokens over a paged K/V cache: the C entry point, its checks, the launch and its tensor maps.
 #include <algorithm>
-#include <atomic>
 #include <cmath>
-#include <cstring>
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 #include "fa_internal.h"
 #include "fa_paged.h"
 #include "paged_kernels.h"
 #include "paged_plan.cuh"
-#include "sm100_ptx.cuh"
 
 namespace fa {
 
@@ -186,6 +181,14 @@ int output_map(CUtensorMap* m, const fa_paged_fwd_params* p) {
 
 using namespace fa;
 
+#ifdef FA_TEST_SHORT_WAIT
+static int test_leave_out = -1;
+extern "C" int fa_test_leave_out_paged_tiles(int n) {
+    test_leave_out = n;
+    return 0;
+}
+#endif
+
 extern "C" {
 
 size_t fa_paged_fwd_workspace_bytes(const fa_paged_fwd_params* p) {
@@ -235,6 +238,9 @@ int fa_paged_fwd(const fa_paged_fwd_params* p) {
     a.o_tma = a.o_units && !a.o_is_fp32 && 32 % a.plan.group == 0 && p->o_stride[0] < (1LL << 39) && p->o_stride[1] * a.plan.group < (1LL << 39) &&
               p->o_stride[0] >= 0 && p->o_stride[1] >= 0;
     a.status = p->status;
+#ifdef FA_TEST_SHORT_WAIT
+    a.leave_out = test_leave_out;
+#endif
     cudaStream_t stream = static_cast<cudaStream_t>(p->stream);
     const bool bf16 = c.dtype == FA_DTYPE_BF16;
     CUtensorMap tq, tk, tv, to = {};

@@ -260,6 +260,10 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
             const int* table = a.page_table + g.b * a.table_stride;
             for (int t = 0; t < chunk_tiles(tiles, c); ++t) {
                 const int st = slot % kStages, tile = tile0 + t;
+                if (left_out(a, slot)) {
+                    ++slot;
+                    continue;
+                }
                 bool bad = false;
                 const int page = page_lookup(a, mine, table, tile, vis_lo, vis_hi, &bad);
                 if (__any_sync(0xffffffffu, bad) && lane == 0) {

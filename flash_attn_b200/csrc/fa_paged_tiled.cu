@@ -215,6 +215,7 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             };
             int tt = 0, parts_with_tiles = 0;
             for (int nth = 0;; ++nth) {
+                if (fail == 0 && __any_sync(0xffffffffu, *abort_flag != 0)) fail = 1;  // (no more than what was taken)
                 if (nth > 0) {
                     ask();
                     answer();
@@ -246,6 +247,7 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                 };
                 const int token0 = token_of(g), hi = g.lo + g.n_tiles;
                 for (int t = 0; t < g.n_tiles && fail == 0; ++t, ++tt) {  // KV tiles are walked from the last to the first
+                    if (left_out(a, tt)) continue;
                     const int st = tt % C::kStages;
                     const uint32_t ph = (tt / C::kStages) & 1;
                     const int tile = hi - 1 - t, page = lookup(tile);

@@ -44,6 +44,9 @@ struct PagedArgs {
     float2* ml_partial;       // [parts of split items][plan.rows]: maximum (log2 units) and sum
     unsigned long long* counts;  // [parts of split items]: those of an item's first part are its count
     int* status;
+#ifdef FA_TEST_SHORT_WAIT
+    int leave_out;            // test build only: the first CTA loads no tile of its stream from this one on; -1: it loads them all
+#endif
 };
 
 // columns: rows of a block, 1, 4, 8 or 16.
@@ -102,6 +105,14 @@ __device__ __forceinline__ void page_load(const PagedArgs& a, const PageBoxes& b
                     head * box.head_coord);
     else
         tma_load_4d(dst + p.to, map, bar, p.column, slot, head, page);
+}
+// Test build only (-DFA_TEST_SHORT_WAIT): whether tile n of the CTA's stream is not loaded, so that the bounded waits behind it run out.
+__device__ __forceinline__ bool left_out(const PagedArgs& a, int n) {
+#ifdef FA_TEST_SHORT_WAIT
+    return blockIdx.x == 0 && a.leave_out >= 0 && n >= a.leave_out;
+#else
+    return false;
+#endif
 }
 // Zeros over the rows of a tile outside [head, tail), by a warp.
 template <int kHalves>

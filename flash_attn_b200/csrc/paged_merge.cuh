@@ -22,7 +22,7 @@ __device__ __forceinline__ bool last_to_come(const PagedArgs& a, int slot, int p
 // microsecond for 128 KB.
 template <int D, bool kBf16, int kWarps, int kRows>
 __device__ __forceinline__ void merge_parts(const PagedArgs& a, int slot, int parts, int head_k, int first, int row0, int n_rows, int warp) {
-    constexpr int kUnroll = kRows > 4 ? 2 : 16 / kRows;
+    constexpr int kUnroll = 16 / kRows;
     const int lane = threadIdx.x & 31;
     const bool mine = lane * 4 < D;
     for (int k0 = warp * kRows; k0 < n_rows; k0 += kWarps * kRows) {
