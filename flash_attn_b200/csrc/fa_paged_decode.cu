@@ -1,13 +1,16 @@
 // Attention of few rows a sequence over a paged K/V cache (single tokens, the check of guessed tokens): HBM-bound, each K/V byte used
 // once.
 //
-// A CTA walks parts of the keys of blocks of rows, one behind the other (paged_parts.cuh).  The operands are swapped, as in the decode kernel for
-// contiguous K/V, so that the 128 lanes of tensor memory hold KEYS:
+// A CTA walks parts of the keys of blocks of rows, one behind the other (paged_parts.cuh).  The operands are swapped, as in the decode
+// kernel for contiguous K/V, so that the 128 lanes of tensor memory hold KEYS:
 //     S^T[128 keys x 16] = K_tile[128 x d] * Q^T[d x 16],   O^T[d x 16] += V_tile^T[d x 128 keys] * P[128 keys x 16]
 // with the block's rows (a row is a token and a query head; the heads of a K/V head lie side by side) in the first kH columns.
 // A tile of 128 keys is 128 / page_size pages, or a part of one: a lane of the producer warp looks a page up and issues its box, so
 // that all boxes of a tile leave in one instruction and the lookup's latency hides behind the wait for a free slot.  Pages of which
 // no row sees a key are not looked up.
+//
+// [64 x 32 heads on 8, 8192 keys each, d 128]: 322 us with pages of 16 tokens, 6.7 TB/s; 100 .. 8192 keys: 82 us, 5.4 TB/s (set-up 5 us, the
+// last parts 8); one sequence of 1000 keys: 13 us.  The code is kept short on purpose: what runs once is fetched from HBM first.
 //
 // What the pool holds beyond a sequence is not known, and 0 * NaN is NaN: keys that no row sees have P = 0 by their scores, and
 // their rows of a V tile are overwritten with zeros before its MMAs, on the first and last tile of a block.

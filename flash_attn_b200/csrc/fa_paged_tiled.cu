@@ -1,8 +1,9 @@
 // Attention of chunks of new tokens over a paged K/V cache: tensor-bound.
 //
-// A CTA walks parts of the keys of blocks of rows, one behind the other (paged_parts.cuh); a block is NQ query tiles of 128 rows.  A row is a token and a query head:
-// the heads of a K/V head lie side by side in a tile (row = token * group + head, as one TMA box of Q lands), so that they share every
-// K/V tile and a few tokens fill it; where the group does not divide 128 the tile's last rows are left over.
+// A CTA walks parts of the keys of blocks of rows, one behind the other (paged_parts.cuh); a block is NQ query tiles of 128 rows.  A
+// row is a token and a query head: the heads of a K/V head lie side by side in a tile (row = token * group + head, as one TMA box of Q
+// lands), so that they share every K/V tile and a few tokens fill it; where the group does not divide 128 the tile's last rows are
+// left over.
 // The walk is the tiled kernel's for contiguous K/V: a TMA warp feeds a ring of K/V tiles, an MMA warp issues S = Q K^T into tensor
 // memory, four softmax warps a query tile keep a row a thread, write P over S, and the MMA warp adds P V; two query tiles alternate
 // on the tensor pipe.  A KV tile is 128 / page_size pages (or a part of one), a box each, looked up and issued by a lane each.
@@ -10,6 +11,9 @@
 //
 // What the pool holds beyond a sequence is not known, and 0 * NaN is NaN: rows of a V tile that no row of the block sees are
 // overwritten with zeros before its MMAs (first and last tile only).
+//
+// 2048 tokens over 32768 keys, 32 heads on 8, d 128: 960 us, 1.1 PFLOP/s, a KV tile of two query tiles 1.8 to 2.1 us (a chain of latencies of two
+// softmax warps a scheduler); six prompts of 200 .. 2048 tokens: 43 us, where parts of one to eight tiles begin and end.
 #include <algorithm>
 #include <atomic>
 #include <cuda_bf16.h>
