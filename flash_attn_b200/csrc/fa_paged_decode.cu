@@ -230,31 +230,29 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
             __syncwarp();
             return have ? g.n_tiles : -1;
         };
-        // The tiles of the next part that has any, -1: there is none.  false: a wait gave up.
+        // The tiles of the next part (there may be none of them), -1: there is no other part.  false: a wait gave up.
         auto next_part = [&](int* tiles) -> bool {
-            for (;;) {
-                if (nth > 0) {
-                    ask();
-                    if (asked > answered && !answer(abort_flag)) return false;
-                }
-                owed = index >= 0;
-                const int at = nth % kSegs;
-                if (nth >= kSegs && !mbar_wait_warp_ok(bar_seg_free + 8 * at, (nth / kSegs - 1) & 1, abort_flag)) return false;
-                *tiles = find(at);
-                owed = false;
-                while (*tiles < 0 && index >= 0) {  // CTAs behind the last part need not start
-                    ask();
-                    if (!answer(abort_flag)) return false;
-                }
-                if (lane == 0) {
-                    bad_seg[at] = 0;
-                    *handed_on = nth + 1;
-                    mbar_arrive(bar_seg_full + 8 * at);
-                }
-                __syncwarp();
-                ++nth;
-                if (*tiles != 0) return true;
+            if (nth > 0) {
+                ask();
+                if (asked > answered && !answer(abort_flag)) return false;
             }
+            owed = index >= 0;
+            const int at = nth % kSegs;
+            if (nth >= kSegs && !mbar_wait_warp_ok(bar_seg_free + 8 * at, (nth / kSegs - 1) & 1, abort_flag)) return false;
+            *tiles = find(at);
+            owed = false;
+            while (*tiles < 0 && index >= 0) {  // CTAs behind the last part need not start
+                ask();
+                if (!answer(abort_flag)) return false;
+            }
+            if (lane == 0) {
+                bad_seg[at] = 0;
+                *handed_on = nth + 1;
+                mbar_arrive(bar_seg_full + 8 * at);
+            }
+            __syncwarp();
+            ++nth;
+            return true;
         };
         int slot = 0;
         auto push_chunk = [&](bool of_k, int part, int tiles, int c) -> bool {
@@ -303,7 +301,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
             copies_arrive(bar_q_full + 8 * buf);
             return true;
         };
-        // The K tiles are a chunk ahead of the V tiles: part, its tiles, chunk; K's part among those with tiles.
+        // The K tiles are a chunk ahead of the V tiles: part, its tiles, chunk; K's part among those with tiles.  A part without tiles
+        // takes a turn of each, in which nothing is loaded: were several handed on in one turn, the ring could be full of them while
+        // the last V tiles of the part before, which its oldest place waits for, are still to be issued.
         int k_part = 0, k_tiles = 0, ck = 0, v_part = 0, v_tiles = -1, cv = 0, nk = -1;
         bool ok = true;
         while (ok && (k_tiles >= 0 || v_tiles >= 0)) {
@@ -311,14 +311,14 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
                 ok = next_part(&k_tiles);
                 ck = 0;
                 k_part = nth - 1;
-                if (ok && k_tiles >= 0) ok = push_q(k_part, ++nk);
+                if (ok && k_tiles > 0) ok = push_q(k_part, ++nk);
             }
             // (the answer is here when it is needed, and a long part leaves the next to who is sooner done)
             if (ok && k_tiles >= 0 && (ck + 1) * kChunkTiles >= k_tiles) ask();
 #pragma unroll 1
             for (int kv = 0; kv < 2; ++kv) {
                 const bool of_k = kv == 0;
-                if (ok && (of_k ? k_tiles : v_tiles) >= 0) ok = push_chunk(of_k, of_k ? k_part : v_part, of_k ? k_tiles : v_tiles, of_k ? ck : cv);
+                if (ok && (of_k ? k_tiles : v_tiles) > 0) ok = push_chunk(of_k, of_k ? k_part : v_part, of_k ? k_tiles : v_tiles, of_k ? ck : cv);
             }
             if (v_tiles < 0 || ++cv * kChunkTiles >= v_tiles) {
                 v_part = k_part;
@@ -414,19 +414,14 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
         bool ok = true;
         while (ok && (k_tiles >= 0 || v_tiles >= 0)) {
             if (k_tiles >= 0 && ++ck * kChunkTiles >= k_tiles) {
-                for (;;) {
-                    ++k_part;
-                    ok = mbar_wait_warp_ok(bar_seg_full + 8 * (k_part % kSegs), (k_part / kSegs) & 1, abort_flag);
-                    if (!ok) break;
-                    k_tiles = segs[k_part % kSegs].n_rows > 0 ? segs[k_part % kSegs].n_tiles : -1;
-                    if (k_tiles != 0) break;
-                    free_part(k_part);
-                }
+                ++k_part;
+                ok = mbar_wait_warp_ok(bar_seg_full + 8 * (k_part % kSegs), (k_part / kSegs) & 1, abort_flag);
+                if (ok) k_tiles = segs[k_part % kSegs].n_rows > 0 ? segs[k_part % kSegs].n_tiles : -1;
                 ck = 0;
-                ++nk;
+                if (k_tiles > 0) ++nk;
             }
-            if (ok && k_tiles >= 0) ok = qk_chunk(k_tiles, ck, nk);
-            if (ok && v_tiles >= 0) ok = pv_chunk(v_part, v_tiles, cv);
+            if (ok && k_tiles > 0) ok = qk_chunk(k_tiles, ck, nk);
+            if (ok && v_tiles > 0) ok = pv_chunk(v_part, v_tiles, cv);
             if (v_tiles < 0 || ++cv * kChunkTiles >= v_tiles) {
                 if (v_tiles >= 0) free_part(v_part);
                 v_part = k_part;
