@@ -112,7 +112,8 @@ TEST_LIB = os.path.join(PKG, "libfa_b200_shortwait.so")
 def build_test_variant(force=False):
     """Builds libfa_b200_shortwait.so, the library compiled with -DFA_TEST_SHORT_WAIT: bounded waits give
     up after about 2 ms and the producers can be told to leave KV tiles out
-    (fa_test_skip_kv_tile, fa_test_skip_decode_tile, fa_test_leave_out_paged_tiles).  Used only by the GPU test of the give-up path."""
+    (fa_test_skip_kv_tile, fa_test_skip_decode_tile, fa_test_leave_out_paged_tiles); it can also be asked for the parts of a launch over
+    the paged cache (fa_test_paged_parts).  Used only by GPU tests."""
     if force or needs_build(TEST_LIB):
         _compile(TEST_LIB, os.path.join(PKG, "build", "shortwait"), ["-DFA_TEST_SHORT_WAIT"])
     return TEST_LIB

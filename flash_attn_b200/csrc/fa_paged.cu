@@ -5,6 +5,9 @@
 #include "fa_paged.h"
 #include "paged_kernels.h"
 #include "paged_plan.cuh"
+#ifdef FA_TEST_SHORT_WAIT
+#include "paged_parts.cuh"
+#endif
 
 namespace fa {
 
@@ -89,6 +92,29 @@ PagedLaunch plan_launch(const fa_paged_fwd_params* p, int sms) {
     l.o_bytes = room(static_cast<size_t>(l.partials) * l.rows * l.wide * sizeof(float));
     if (l.partials > 0) l.bytes = l.count_bytes + l.ml_bytes + l.o_bytes;
     return l;
+}
+
+PagedPlan plan_of(const fa_paged_fwd_params* p, const PagedLaunch& l) {
+    const fa_paged_kv& c = p->cache;
+    PagedPlan x = {};
+    x.seq = {c.seqlens_k, c.cu_seqlens_q, c.batch, static_cast<int>(p->tokens)};
+    x.heads_k = c.heads;
+    x.group = p->heads / c.heads;
+    x.rows = l.rows;
+    x.block_tokens = l.rows / x.group + 2;  // (it may begin and end inside a token)
+    x.div_rows = make_fastdiv(static_cast<uint32_t>(l.rows));
+    x.is_causal = p->is_causal ? 1 : 0;
+    // (a window of 2^29 or more hides nothing that the cache could hold)
+    x.window_left = p->window_left < kMostKeys / 2 ? p->window_left : -1;
+    x.window_right = p->window_right < kMostKeys / 2 ? p->window_right : -1;
+    x.slots = l.slots;
+    x.min_share = l.min_share;
+    x.long_share = l.long_share;
+    x.waves = l.waves;
+    x.one_wave = l.columns ? kDecodeOneWave : kOneWave;
+    x.most_parts = l.most_parts;
+    x.partials = static_cast<int>(l.partials);
+    return x;
 }
 
 // A tensor map: extents, strides (elements; of a dimension of one any will do) and box, innermost first.  The last ones are kept per
@@ -187,6 +213,35 @@ extern "C" int fa_test_leave_out_paged_tiles(int n) {
     test_leave_out = n;
     return 0;
 }
+
+// The parts of a call as its producers find them, asked for in any order: out[i] = part order[i], n_rows = 0 where there is none.
+// Device memory both; sizes: those of the launch (numbers of parts at most, room for partial rows, SMs' worth of CTAs).
+static __global__ void test_parts(const PagedPlan plan, const FastDiv div_group, const int* order, int n, PagedSeg* out) {
+    const int lane = threadIdx.x;
+    long long tiles = 0;
+    for (int b = lane; b < plan.seq.batch; b += 32) {
+        const int2 x = blocks_and_tiles(plan, seq_span(plan.seq, b));
+        tiles += static_cast<long long>(x.x) * x.y;
+    }
+    PartLine line;
+    line.start(plan, lane, sum_all(tiles) * plan.heads_k);
+    for (int i = 0; i < n; ++i) {
+        PagedSeg g = {};
+        if (!line.find(plan, div_group, order[i], lane, &g)) g.n_rows = 0;
+        if (lane == 0) out[i] = g;
+        __syncwarp();
+    }
+}
+extern "C" int fa_test_paged_parts(const fa_paged_fwd_params* p, const int* order, int n, void* out, int64_t* sizes) {
+    int sms = 0, major = 0, rc = check_fwd(p);
+    if (rc != FA_OK || (rc = current_device(&sms, &major)) != FA_OK) return rc;
+    const PagedLaunch l = plan_launch(p, sms);
+    sizes[0] = l.grid;
+    sizes[1] = l.partials;
+    sizes[2] = l.slots;
+    if (n > 0) test_parts<<<1, 32, 0, static_cast<cudaStream_t>(p->stream)>>>(plan_of(p, l), make_fastdiv(static_cast<uint32_t>(p->heads / p->cache.heads)), order, n, static_cast<PagedSeg*>(out));
+    return cudaGetLastError() == cudaSuccess ? FA_OK : FA_ERR_CUDA;
+}
 #endif
 
 extern "C" {
@@ -210,13 +265,7 @@ int fa_paged_fwd(const fa_paged_fwd_params* p) {
     if (l.bytes > 0 && (reinterpret_cast<uintptr_t>(p->workspace) & 15u)) return FA_ERR_INVALID_ARG;
     const fa_paged_kv& c = p->cache;
     PagedArgs a = {};
-    a.plan.seq = {c.seqlens_k, c.cu_seqlens_q, c.batch, static_cast<int>(p->tokens)};
-    a.plan.heads_k = c.heads;
-    a.plan.group = p->heads / c.heads;
-    a.plan.is_causal = p->is_causal ? 1 : 0;
-    // (a window of 2^29 or more hides nothing that the cache could hold)
-    a.plan.window_left = p->window_left < kMostKeys / 2 ? p->window_left : -1;
-    a.plan.window_right = p->window_right < kMostKeys / 2 ? p->window_right : -1;
+    a.plan = plan_of(p, l);
     a.div_group = make_fastdiv(static_cast<uint32_t>(a.plan.group));
     a.q = p->q;
     a.o = p->o;
@@ -245,16 +294,6 @@ int fa_paged_fwd(const fa_paged_fwd_params* p) {
     const bool bf16 = c.dtype == FA_DTYPE_BF16;
     CUtensorMap tq, tk, tv, to = {};
     if ((rc = page_maps(&tk, &tv, c, &a)) != FA_OK) return rc;
-    a.plan.rows = l.rows;
-    a.plan.block_tokens = l.rows / a.plan.group + 2;  // (it may begin and end inside a token)
-    a.plan.div_rows = make_fastdiv(static_cast<uint32_t>(l.rows));
-    a.plan.slots = l.slots;
-    a.plan.min_share = l.min_share;
-    a.plan.long_share = l.long_share;
-    a.plan.waves = l.waves;
-    a.plan.most_parts = l.most_parts;
-    a.plan.one_wave = l.columns ? kDecodeOneWave : kOneWave;
-    a.plan.partials = static_cast<int>(l.partials);
     if (l.bytes > 0) {
         char* room = static_cast<char*>(p->workspace);
         a.counts = reinterpret_cast<unsigned long long*>(room);

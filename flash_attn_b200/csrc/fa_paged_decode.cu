@@ -239,10 +239,11 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
             owed = index >= 0;
             const int at = nth % kSegs;
             if (nth >= kSegs && !mbar_wait_warp_ok(bar_seg_free + 8 * at, (nth / kSegs - 1) & 1, abort_flag)) return false;
-            *tiles = find(at);
-            owed = false;
-            while (*tiles < 0 && index >= 0) {  // CTAs behind the last part need not start
-                ask();
+            for (;;) {
+                *tiles = find(at);
+                owed = false;
+                if (*tiles >= 0 || index < 0) break;
+                ask();  // a CTA behind the last part need not start; one before it may still be taken
                 if (!answer(abort_flag)) return false;
             }
             if (lane == 0) {

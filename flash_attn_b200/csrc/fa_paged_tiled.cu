@@ -227,7 +227,13 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                 const int at = nth % kSegs;
                 if (nth >= kSegs && !wait_part(bar_seg_free + 8 * at, (nth / kSegs - 1) & 1)) { fail = 3; break; }
                 PagedSeg g;
-                const bool have = index >= 0 && line.find(a.plan, a.div_group, index, lane, &g);
+                bool have;
+                for (;;) {
+                    have = index >= 0 && line.find(a.plan, a.div_group, index, lane, &g);
+                    if (have || index < 0) break;
+                    ask();  // a CTA behind the last part need not start; one before it may still be taken
+                    answer();
+                }
                 if (!have) g.n_rows = 0;
                 if (lane == 0) {
                     segs[at] = g;
@@ -235,13 +241,7 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                     mbar_arrive(bar_seg_full + 8 * at);
                 }
                 __syncwarp();
-                if (!have) {
-                    while (index >= 0) {  // CTAs behind the last part need not start
-                        ask();
-                        answer();
-                    }
-                    break;
-                }
+                if (!have) break;
                 if (g.n_tiles == 0) continue;
                 const int* table = a.page_table + g.b * a.table_stride;
                 bool met_bad = false;

@@ -10,7 +10,7 @@
 // Long parts have the lower numbers, so that the short ones fill what the long ones leave at the end.
 //
 // The lengths of all sequences are read by one warp, which knows where the parts of each begin from a scan over them, 32 sequences at a
-// time; a later part is looked for from the one before on.
+// time; a later part is looked for from the one before on, an earlier one (nothing says in which order CTAs are taken) from the start.
 #pragma once
 #include "paged_kernels.h"
 
@@ -112,8 +112,15 @@ struct PartLine {
         base = 0;
         count(p, lane);
     }
-    // Part `nth` of all (once there was none, there is none; no less than the one asked for before); false: there are not so many.
+    // Part `nth` of all; false: there are not so many.
     __device__ __forceinline__ bool find(const PagedPlan& p, const FastDiv& div_group, int nth, int lane, PagedSeg* g) {
+        if (nth < static_cast<long long>(static_cast<unsigned>(base))) {  // (of sequences that the scan has left behind)
+            b0 = pass = 0;
+            base = 0;
+            if (p.seq.batch > 32) read(p, lane);
+            count(p, lane);
+        }
+        if (pass >= passes) return false;  // (base: of all)
         for (;;) {
             const long long sum = __shfl_sync(0xffffffffu, upto, 31);
             if (nth < static_cast<long long>(static_cast<unsigned>(base + sum))) break;

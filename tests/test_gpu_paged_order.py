@@ -1,0 +1,65 @@
+"""The parts of a launch over the paged cache: each is found by its number whatever was asked for before (CTAs are taken in no
+promised order), and together they are every item's keys, once."""
+import random
+
+import pytest
+import torch
+
+import paged_parts_util as pp
+import paged_util as pu
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def L():
+    return pp.test_library()
+
+
+def batches():
+    r = random.Random(5)
+    yield "long single tokens", [1] * 3, [9000, 40, 30000], 8, 2, 128
+    yield "single tokens, a warp's sequences", [1] * 32, [r.randint(1, 9000) for _ in range(32)], 16, 4, 64
+    yield "single tokens, more of them", [1] * 100, [r.randint(0, 9000) for _ in range(100)], 8, 8, 128
+    yield "single tokens, a block's sequences", [1] * 700, [r.choice([0, 3, 200, r.randint(1, 5000)]) for _ in range(700)], 8, 2, 64
+    yield "guessed tokens", [5] * 40, [r.randint(5, 6000) for _ in range(40)], 4, 4, 128
+    yield "chunks", [r.randint(0, 300) for _ in range(20)], [r.randint(300, 9000) for _ in range(20)], 8, 1, 128
+    yield "chunks beside single tokens", [700] + [1] * 50, [9000] + [r.randint(1, 4000) for _ in range(50)], 7, 1, 64
+
+
+@pytest.mark.parametrize("lens_q, lens_k, H, Hk, d", [x[1:] for x in batches()], ids=[x[0] for x in batches()])
+@pytest.mark.parametrize("window", [(-1, -1), (1000, -1)])
+def test_parts_are_found_in_any_order(L, lens_q, lens_k, H, Hk, d, window):
+    lens, cu = torch.tensor(lens_k, dtype=torch.int32).cuda(), pu.cumulated(lens_q)
+    p = pp.params(sum(lens_q), H, Hk, d, lens, cu, max(lens_q), -(-max(lens_k) // 16), window=window)
+    found, grid, room, slots = pp.parts(L, p)
+    count = sum(x is not None for x in found)
+    assert 0 < count <= grid and all(x is not None for x in found[:count])
+    # every item's rows and tiles, once
+    items = {}
+    for x in found[:count]:
+        items.setdefault((x["b"], x["head"], x["row0"]), []).append(x)
+    rows, taken = {}, set()
+    for (b, head, _), of in items.items():
+        assert [x["part"] for x in sorted(of, key=lambda x: x["part"])] == list(range(of[0]["parts"]))
+        of.sort(key=lambda x: x["part"])
+        at = of[0]["lo"]
+        for x in of:
+            assert (x["slot"], x["parts"], x["n_rows"], x["vis_lo"], x["vis_hi"]) == tuple(of[0][k] for k in ("slot", "parts", "n_rows", "vis_lo", "vis_hi"))
+            assert x["lo"] == at
+            at += x["n_tiles"]
+        lo, hi = of[0]["vis_lo"], of[0]["vis_hi"]
+        assert sum(x["n_tiles"] for x in of) == (-(-hi // 128) - lo // 128 if hi > lo else 0)
+        rows[b, head] = rows.get((b, head), 0) + of[0]["n_rows"]
+        if of[0]["parts"] > 1:
+            places = set(range(of[0]["slot"], of[0]["slot"] + of[0]["parts"]))
+            assert not places & taken and max(places) < room
+            taken |= places
+    assert rows == {(b, h): n * (H // Hk) for b, n in enumerate(lens_q) if n for h in range(Hk)}
+    # the same whatever comes before
+    r = random.Random(1)
+    orders = [list(reversed(range(len(found)))), r.sample(range(len(found)), len(found)), [r.randrange(len(found)) for _ in range(500)],
+              [len(found) - 1, 0, len(found) - 1, count - 1, count, 0, count // 2]]
+    for order in orders:
+        again, *_ = pp.parts(L, p, order)
+        assert again == [found[i] for i in order]
