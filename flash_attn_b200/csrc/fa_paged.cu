@@ -114,6 +114,7 @@ PagedPlan plan_of(const fa_paged_fwd_params* p, const PagedLaunch& l) {
     x.one_wave = l.columns ? kDecodeOneWave : kOneWave;
     x.most_parts = l.most_parts;
     x.partials = static_cast<int>(l.partials);
+    x.grid = static_cast<int>(std::min(l.grid, 0x7fffffffLL));  // (a larger one is refused)
     return x;
 }
 

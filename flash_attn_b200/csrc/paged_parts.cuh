@@ -48,6 +48,10 @@ __device__ __forceinline__ long long sum_all(long long v) {
 }
 __device__ __forceinline__ void prefetch_l1(const void* p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(p)); }
 
+// Parts are counted in 36 bits: 32 sequences of 2^30 blocks each, which cu_seqlens_q that go back and forth can come to.
+constexpr int kPartBits = 36;
+__device__ __forceinline__ long long part_count(long long x) { return x & ((1LL << kPartBits) - 1); }
+
 // The parts of a launch, by one warp.
 struct PartLine {
     int share;
@@ -55,7 +59,7 @@ struct PartLine {
     int b0, pass, passes, parts;
     SeqSpan s;
     int2 x;                  // blocks, tiles
-    long long own, upto;     // parts of the lane's sequence (and in the upper half those of split items), and of the lanes up to it
+    long long own, upto;     // parts of the lane's sequence (and above kPartBits those of split items), and of the lanes up to it
     long long base;          // of the sequences before b0
 
     __device__ __forceinline__ void read(const PagedPlan& p, int b) {
@@ -71,7 +75,7 @@ struct PartLine {
             size = longest * 2 > share ? 0 : longest * 4 > share ? 1 : kSizes - 1;
         }
         own = size == pass ? static_cast<long long>(x.x) * p.heads_k * parts : 0;
-        if (parts > 1) own |= own << 32;
+        if (parts > 1) own |= own << kPartBits;  // (fewer than 2 waves * slots of all)
         upto = scan_add(own, lane);
     }
     // tiles: of all sequences and K/V heads, where the block has added them up (more than kWarpSeqs sequences).
@@ -112,9 +116,11 @@ struct PartLine {
         base = 0;
         count(p, lane);
     }
-    // Part `nth` of all; false: there are not so many.
+    // Part `nth` of all; false: there are not so many, or it belongs to an item that the launch has no CTAs or no room for.  (Rows that
+    // several sequences claim are more than the launch was made for: such an item is left out with all of its parts.)
     __device__ __forceinline__ bool find(const PagedPlan& p, const FastDiv& div_group, int nth, int lane, PagedSeg* g) {
-        if (nth < static_cast<long long>(static_cast<unsigned>(base))) {  // (of sequences that the scan has left behind)
+        if (nth >= p.grid) return false;
+        if (nth < part_count(base)) {  // (of sequences that the scan has left behind)
             b0 = pass = 0;
             base = 0;
             if (p.seq.batch > 32) read(p, lane);
@@ -123,7 +129,7 @@ struct PartLine {
         if (pass >= passes) return false;  // (base: of all)
         for (;;) {
             const long long sum = __shfl_sync(0xffffffffu, upto, 31);
-            if (nth < static_cast<long long>(static_cast<unsigned>(base + sum))) break;
+            if (nth < part_count(base + sum)) break;
             base += sum;
             b0 += 32;
             if (b0 >= p.seq.batch) {
@@ -134,11 +140,10 @@ struct PartLine {
             count(p, lane);
         }
         const long long before = base + upto - own;
-        int at = nth - static_cast<int>(static_cast<unsigned>(before));
-        const unsigned owner = __ballot_sync(0xffffffffu, at >= 0 && at < static_cast<int>(static_cast<unsigned>(own)));
+        const unsigned owner = __ballot_sync(0xffffffffu, nth >= part_count(before) && nth < part_count(before + own));
         const int src = __ffs(owner) - 1;
-        at = __shfl_sync(0xffffffffu, at, src);
-        g->slot = __shfl_sync(0xffffffffu, static_cast<int>(before >> 32), src) + at;
+        const int at = __shfl_sync(0xffffffffu, nth - static_cast<int>(part_count(before)), src);
+        g->slot = __shfl_sync(0xffffffffu, static_cast<int>(before >> kPartBits), src) + at;
         g->b = b0 + src;
         g->first = __shfl_sync(0xffffffffu, s.first, src);
         g->n = __shfl_sync(0xffffffffu, s.end, src) - g->first;
@@ -147,6 +152,7 @@ struct PartLine {
         const int item = static_cast<int>(static_cast<unsigned>(at) / static_cast<unsigned>(g->parts));
         g->part = at - item * g->parts;
         g->slot -= g->part;
+        if (g->parts > p.grid - (nth - g->part) || (g->parts > 1 && g->parts > p.partials - g->slot)) return false;
         const int blocks = __shfl_sync(0xffffffffu, x.x, src);
         g->head = static_cast<int>(static_cast<unsigned>(item) / static_cast<unsigned>(blocks));
         const int blk = item - g->head * blocks;

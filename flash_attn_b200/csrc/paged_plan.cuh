@@ -24,6 +24,7 @@ struct PagedPlan {
     int one_wave;         // tiles a slot up to which all parts are to run at once
     int most_parts;       // of an item: as many as the table's width gives (a length may be beyond it)
     int partials;         // parts of split items that there is room for (0: nothing is split)
+    int grid;             // parts that there are CTAs for
 };
 
 #ifdef __CUDACC__

@@ -313,6 +313,7 @@ int fa_ring_comm_destroy(void* comm);
  * call is replayed on new ones.
  * Whatever they hold, no memory outside the tensors is touched: a negative length counts as 0, row numbers are clipped
  * to the rows there are, and a page that is not in the pool (or beyond the table's width) is never followed: see status.
+ * (Where cu_seqlens_q does not ascend, rows that several sequences claim get what one of them gives, or stay as they were.)
  * Slots at or past seqlens_k[b], and pages of which no row sees a key, may hold anything.
  */
 typedef struct fa_paged_kv {

@@ -63,3 +63,48 @@ def test_parts_are_found_in_any_order(L, lens_q, lens_k, H, Hk, d, window):
     for order in orders:
         again, *_ = pp.parts(L, p, order)
         assert again == [found[i] for i in order]
+
+
+# cu_seqlens_q that go back and forth: every other sequence claims the same rows, which is more than a launch is sized for
+@pytest.mark.parametrize("T, H, Hk, batch, keys, most", [(1, 1, 1, 32, 8192, 1), (1, 1, 1, 200, 8192, 1), (1, 4, 1, 700, 4096, 1), (5, 4, 4, 31, 9000, 5),
+                                                         (300, 8, 2, 30, 9000, 300), (300, 8, 2, 600, 3000, 300), (2000, 4, 1, 400, 2500, 2000)])
+def test_rows_that_many_sequences_claim_stay_inside_the_workspace(L, T, H, Hk, batch, keys, most):
+    lens = torch.full((batch,), keys, dtype=torch.int32, device="cuda")
+    cu = torch.tensor([T * (i % 2) for i in range(batch + 1)], dtype=torch.int32).cuda()
+    p = pp.params(T, H, Hk, 64, lens, cu, most, -(-keys // 16))
+    found, grid, room, _ = pp.parts(L, p)
+    seen = {}
+    for x in found:
+        if x is not None:
+            assert x["parts"] == 1 or 0 <= x["slot"] <= room - x["parts"]
+            seen.setdefault((x["b"], x["head"], x["row0"]), []).append(x["part"])
+            seen[x["b"], x["head"], x["row0"], "of"] = x["parts"]
+    assert any(x is not None for x in found) and all(x is None for x in found[grid:])
+    for item, of in seen.items():
+        if len(item) == 3:  # an item is done with all of its parts, or not at all
+            assert sorted(of) == list(range(seen[(*item, "of")]))
+
+
+@pytest.mark.parametrize("T, H, Hk, batch, keys, most", [(1, 1, 1, 32, 8192, 1), (1, 4, 1, 700, 4096, 1), (300, 8, 2, 30, 9000, 300), (5, 4, 4, 31, 9000, 5)])
+def test_a_workspace_outlives_rows_that_many_sequences_claim(T, H, Hk, batch, keys, most):
+    import ctypes
+
+    import flash_attn_b200 as fa
+    from flash_attn_b200 import _lib
+    t, d = torch.bfloat16, 64
+    k, v, one = pu.make_cache([keys], 16, Hk, d, t, seed=1)
+    table, lens = one.expand(batch, -1).contiguous(), torch.full((batch,), keys, dtype=torch.int32, device="cuda")
+    q = torch.randn(T, H, d, device="cuda").to(t)
+    good = torch.tensor([0] + [T] * batch, dtype=torch.int32).cuda()
+    bad = torch.tensor([T * (i % 2) for i in range(batch + 1)], dtype=torch.int32).cuda()
+    need = _lib.load().fa_paged_fwd_workspace_bytes(ctypes.byref(pp.params(T, H, Hk, d, lens, bad, most, table.shape[1])))
+    assert need > 0
+    room = torch.full((need + (1 << 20),), 0x5a, dtype=torch.uint8, device="cuda")
+    call = lambda cu: fa.paged_attn_forward(q, k, v, table, lens, cu, most, causal=True, workspace=room[:need])  # noqa: E731
+    want = call(good)
+    pu.check_attention(*want, pu.attention(q, k, v, table, [keys], [T], causal=True), t, keys)
+    for _ in range(3):
+        call(bad)
+        got = call(good)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert bool((room[need:] == 0x5a).all())
