@@ -100,6 +100,7 @@ PagedPlan plan_of(const fa_paged_fwd_params* p, const PagedLaunch& l) {
     x.seq = {c.seqlens_k, c.cu_seqlens_q, c.batch, static_cast<int>(p->tokens)};
     x.heads_k = c.heads;
     x.group = p->heads / c.heads;
+    x.table_keys = c.table_width * c.page_size;  // (below kMostKeys)
     x.rows = l.rows;
     x.block_tokens = l.rows / x.group + 2;  // (it may begin and end inside a token)
     x.div_rows = make_fastdiv(static_cast<uint32_t>(l.rows));

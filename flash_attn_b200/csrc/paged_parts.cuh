@@ -21,7 +21,7 @@ struct alignas(16) PagedSeg {
     int b, head, first, n;        // sequence, K/V head, the sequence's first row, new tokens
     int keys, row0, n_rows, part; // keys; rows of the block, inside the sequence (n_rows = 0: there is no other part); part of
     int parts, slot, lo, n_tiles; // the item's parts, and where part 0 leaves its rows
-    int vis_lo, vis_hi, pad[2];   // keys that any of the rows sees
+    int vis_lo, vis_hi, pad[2];   // keys that any of the rows sees (and the table's room, or a key more)
 };
 
 constexpr int kSizes = 3;       // of parts: more than half a share, more than a quarter, less
@@ -161,7 +161,7 @@ struct PartLine {
         const int p_first = g->keys - g->n;
         const int tok_lo = static_cast<int>(fast_div(div_group, static_cast<uint32_t>(g->row0)));
         const int tok_hi = static_cast<int>(fast_div(div_group, static_cast<uint32_t>(g->row0 + g->n_rows - 1)));
-        visible_keys(p, g->keys, p_first + tok_lo, p_first + tok_hi, &g->vis_lo, &g->vis_hi);
+        walked_keys(p, g->keys, p_first + tok_lo, p_first + tok_hi, &g->vis_lo, &g->vis_hi);
         const int tile0 = g->vis_lo / kTile, tiles = g->vis_hi > g->vis_lo ? (g->vis_hi + kTile - 1) / kTile - tile0 : 0;
         int from, to;
         part_of(tiles, g->part, g->parts, &from, &to);

@@ -13,6 +13,7 @@ namespace fa {
 struct PagedPlan {
     SeqTable seq;
     int heads_k, group;
+    int table_keys;       // keys that the page table has room for
     int rows;             // rows of a block
     int block_tokens;     // tokens that a block may reach into
     FastDiv div_rows;
@@ -38,6 +39,12 @@ __device__ __forceinline__ void visible_keys(const PagedPlan& p, int keys, int p
     *hi = max(h, 0);
     *lo = min(l, *hi);
 }
+// And of these the ones to walk: of keys beyond the page table one is kept, by which their rows are known to be without a page (for a
+// length of 2^30 in a table of one page a CTA would walk eight million tiles of nothing).
+__device__ __forceinline__ void walked_keys(const PagedPlan& p, int keys, int p0, int p1, int* lo, int* hi) {
+    visible_keys(p, keys, p0, p1, lo, hi);
+    *hi = min(*hi, max(*lo, p.table_keys) + 1);
+}
 
 // Blocks of a sequence, and the most tiles that one of them walks.
 __device__ __forceinline__ int2 blocks_and_tiles(const PagedPlan& p, const SeqSpan& s) {
@@ -46,7 +53,7 @@ __device__ __forceinline__ int2 blocks_and_tiles(const PagedPlan& p, const SeqSp
     const unsigned rows = static_cast<unsigned>(n) * static_cast<unsigned>(p.group);  // (tokens * heads < 2^30)
     const int blocks = static_cast<int>(fast_div(p.div_rows, rows + p.rows - 1));
     int lo, hi;
-    visible_keys(p, s.keys, s.keys - n, s.keys - 1, &lo, &hi);
+    walked_keys(p, s.keys, s.keys - n, s.keys - 1, &lo, &hi);
     int keys = hi - lo;
     const int right = p.is_causal ? 0 : p.window_right;
     bool cut = false;

@@ -108,3 +108,34 @@ def test_a_workspace_outlives_rows_that_many_sequences_claim(T, H, Hk, batch, ke
         got = call(good)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     assert bool((room[need:] == 0x5a).all())
+
+
+@pytest.mark.parametrize("lens_q, H, Hk, d", [([1, 1, 1], 4, 1, 64), ([3, 1, 2], 4, 2, 128), ([200, 1, 40], 4, 1, 128), ([300, 1, 40], 4, 1, 64)])
+@pytest.mark.parametrize("window", [(-1, -1), (100, -1), (-1, 100)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_a_length_beyond_the_table_costs_no_more_than_the_table(L, lens_q, H, Hk, d, window, causal):
+    """No more tiles than the table has and the first that it lacks; the rows that meet it are NaN, the others as ever."""
+    import flash_attn_b200 as fa
+    t, room = torch.bfloat16, 512
+    cu = pu.cumulated(lens_q)
+    k, v, table = pu.make_cache([room, 300, room], 16, Hk, d, t, seed=2)
+    q = torch.randn(sum(lens_q), H, d, device="cuda").to(t)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for far in (room + 1, room + 150, 10 ** 6, 2 ** 30, 2 ** 31 - 1):
+        lens = torch.tensor([far, 300, room], dtype=torch.int32).cuda()
+        p = pp.params(sum(lens_q), H, Hk, d, lens, cu, max(lens_q), room // 16, causal=causal, window=window)
+        walked = {}
+        for x in pp.parts(L, p)[0]:
+            if x is not None:
+                walked[x["b"], x["head"], x["row0"]] = walked.get((x["b"], x["head"], x["row0"]), 0) + x["n_tiles"]
+        assert max(walked.values()) <= room // 128 + 1
+        status.zero_()
+        o, lse = fa.paged_attn_forward(q, k, v, table, lens, cu, max(lens_q), causal=causal, window=window, status=status)
+        assert int(status) == 400
+        # the last row sees its own place, which the table has no page for (a causal row before the table's end sees none such)
+        assert bool(o[lens_q[0] - 1].isnan().all()) and bool(lse[lens_q[0] - 1].isnan().all())
+        if far >= 10 ** 6:
+            assert bool(o[: lens_q[0]].isnan().all()) and bool(lse[: lens_q[0]].isnan().all())
+        n = lens_q[0]
+        want = pu.attention(q[n:], k, v, table[1:], [300, room], lens_q[1:], causal=causal, window=window)
+        pu.check_attention(o[n:], lse[n:], want, t, room)
