@@ -119,22 +119,22 @@ struct PartLine {
     // Part `nth` of all; false: there are not so many, or it belongs to an item that the launch has no CTAs or no room for.  (Rows that
     // several sequences claim are more than the launch was made for: such an item is left out with all of its parts.)
     __device__ __forceinline__ bool find(const PagedPlan& p, const FastDiv& div_group, int nth, int lane, PagedSeg* g) {
-        if (nth >= p.grid) return false;
-        if (nth < part_count(base)) {  // (of sequences that the scan has left behind)
-            b0 = pass = 0;
-            base = 0;
-            if (p.seq.batch > 32) read(p, lane);
-            count(p, lane);
-        }
-        if (pass >= passes) return false;  // (base: of all)
+        bool again = nth < part_count(base);  // (of sequences that the scan has left behind)
+        if (nth >= p.grid || (!again && pass >= passes)) return false;  // (at the end of the scan, base: of all)
         for (;;) {
-            const long long sum = __shfl_sync(0xffffffffu, upto, 31);
-            if (nth < part_count(base + sum)) break;
-            base += sum;
-            b0 += 32;
-            if (b0 >= p.seq.batch) {
-                if (++pass >= passes) return false;
-                b0 = 0;
+            if (again) {
+                base = 0;
+                b0 = pass = 0;
+                again = false;
+            } else {
+                const long long sum = __shfl_sync(0xffffffffu, upto, 31);
+                if (nth < part_count(base + sum)) break;
+                base += sum;
+                b0 += 32;
+                if (b0 >= p.seq.batch) {
+                    if (++pass >= passes) return false;
+                    b0 = 0;
+                }
             }
             if (p.seq.batch > 32) read(p, b0 + lane);
             count(p, lane);
