@@ -80,20 +80,26 @@ __device__ __forceinline__ int parts_of(const PagedPlan& p, int tiles, int share
 // Each part leaves its rows, un-normalised, with their maxima (log2 units) and sums; then it counts itself in, and the last puts the
 // rows together: O = sum_j 2^(m_j - m) O_j / l, l = sum_j 2^(m_j - m) l_j, in the order of the parts whoever is last.
 //
-// A count needs no clearing before the launch: its upper 48 bits say that it is one.  Whatever else lies there (a workspace that
-// was never used) counts as none come yet, and the last of the parts leaves none come for the next launch.
-constexpr unsigned long long kCountMark = 0x9d3f6ba817c5ull << 16;
+// A count needs no clearing before the launch: that c have come is the word kCountMark + c kCountStep, and whatever else lies there (a
+// workspace that was never used, or that something else has been written to) counts as none come yet.  The last of the parts leaves
+// none come for the next launch.  The step is odd, so that it has an inverse modulo 2^64 and each word stands for one c, of which those
+// below 2^16 are counts: one word of 2^48, and none that differs from a count in one of its four 16-bit pieces (kCountStep^-1 times
+// such a difference is 2^47 or more off zero).
+constexpr unsigned long long kCountMark = 0x9d3f6ba817c50000ull, kCountStep = 0x0fd630f1f29d0da9ull, kCountUnstep = 0xd7da0cbaef15e699ull;
+static_assert(kCountStep * kCountUnstep == 1ull, "inverse modulo 2^64");
+__device__ __forceinline__ unsigned long long come(unsigned long long word) { return (word - kCountMark) * kCountUnstep; }
+constexpr unsigned long long kMostCome = 0xffffull;
 
 // Whether this CTA is the last of its item (one thread, to whom the CTA's partial rows are visible; they are to the others' after).
 __device__ __forceinline__ bool count_in(unsigned long long* count, int parts) {
     __threadfence();
-    unsigned long long was = atomicAdd(count, 1ull);
-    while ((was & ~0xffffull) != kCountMark) {  // not a count: whoever makes it one is the first to come, the others add themselves again
+    unsigned long long was = atomicAdd(count, kCountStep);
+    while (come(was) > kMostCome) {  // not a count: whoever makes it one is the first to come, the others add themselves again
         const unsigned long long seen = *reinterpret_cast<volatile unsigned long long*>(count);
-        if ((seen & ~0xffffull) == kCountMark) was = atomicAdd(count, 1ull);
-        else if (atomicCAS(count, seen, kCountMark | 1ull) == seen) was = kCountMark;  // (ends: a failed exchange is another part's doing)
+        if (come(seen) <= kMostCome) was = atomicAdd(count, kCountStep);
+        else if (atomicCAS(count, seen, kCountMark + kCountStep) == seen) was = kCountMark;  // (ends: a failed exchange is another part's doing)
     }
-    const bool last = static_cast<int>(was & 0xffffull) + 1 == parts;
+    const bool last = static_cast<int>(come(was)) + 1 == parts;
     if (last) {
         *reinterpret_cast<volatile unsigned long long*>(count) = kCountMark;
         __threadfence();

@@ -409,7 +409,8 @@ typedef struct fa_paged_fwd_params {
     int is_causal;
     int window_left, window_right;
     const float* alibi_slopes;/* device fp32 [heads] or NULL */
-    void* workspace;          /* device, 16-byte aligned: partial results of sequences whose keys several CTAs share */
+    void* workspace;          /* device, 16-byte aligned: partial results of sequences whose keys several CTAs share.  It may hold
+                                 anything, except what a call that gave up (300 + n) has left: that is overwritten first, zeros do. */
     size_t workspace_bytes;   /* at least fa_paged_fwd_workspace_bytes(p) */
     int* status;              /* device int or NULL.  FA_STATUS_PAGE: a visible key's page is not in the pool (the rows of the CTAs
                                  that met it are NaN).  300 + n: a bounded wait gave up, as in fa_fwd_params: O and LSE are undefined. */
