@@ -294,6 +294,11 @@ PyObject* forward(PyObject*, PyObject* const* args, Py_ssize_t n) {
 void need_no_grad(const at::Tensor& t, const char* name) {
     if (t.requires_grad() && at::GradMode::is_enabled()) value_error_of(name, "requires grad: call this under torch.no_grad() or inside an autograd Function");
 }
+// float(x) of a number or a tensor of one
+double number_of(PyObject* x, const char* name) {
+    if (THPVariable_Check(x)) need_no_grad(THPVariable_Unpack(x), name);
+    return float_of(x);
+}
 bool sixteen_bit(const at::Tensor& t) { return t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16; }
 void need_rows(const at::Tensor& t, const char* name) {
     if (t.size(-1) > 1 && t.stride(-1) != 1) value_error_of(name, "must be contiguous in its last dimension");
@@ -336,6 +341,7 @@ PyObject* rotary_impl(PyObject* const* args) {
     if ((!one && !each) || (N > 1 && positions.stride(-1) != 1)) value_error("positions must be [seqlen] or [batch, seqlen] ([tokens]), one behind the other");
     if (inv_freq.scalar_type() != at::kDouble || inv_freq.dim() != 1 || !inv_freq.is_contiguous() || inv_freq.numel() < 1 || 2 * inv_freq.numel() > d)
         value_error("inv_freq must be float64 [rotary_dim / 2], rotary_dim at most head_dim");
+    need_no_grad(inv_freq, "inv_freq");
     need_reach(device, positions, "positions");
     need_reach(device, inv_freq, "inv_freq");
     at::Tensor out;
@@ -369,7 +375,7 @@ PyObject* rotary_impl(PyObject* const* args) {
     p.positions_64 = positions.scalar_type() == at::kLong;
     p.position_stride = each ? positions.stride(0) : 0;
     p.inv_freq = static_cast<const double*>(inv_freq.data_ptr());
-    p.amplitude = static_cast<float>(float_of(args[4]));
+    p.amplitude = static_cast<float>(number_of(args[4], "amplitude"));
     p.interleaved = truth_of(args[5]) ? 1 : 0;
     p.inverse = truth_of(args[6]) ? 1 : 0;
     p.stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
@@ -391,6 +397,8 @@ fa_paged_kv cache_of(PyObject* const* args, const at::Tensor& rows, const c10::D
     if (!sixteen_bit(k) || k.scalar_type() != v.scalar_type() || rows.scalar_type() != k.scalar_type())
         value_error("the new tokens and the pages must share dtype float16 or bfloat16");
     if (rows.size(2) != k.size(3)) value_error("the new tokens and the pages must have one head_dim");
+    need_no_grad(k, "k_pages");
+    need_no_grad(v, "v_pages");
     need_rows(k, "k_pages");
     need_rows(v, "v_pages");
     if (table.scalar_type() != at::kInt || table.dim() != 2 || (table.size(1) > 1 && table.stride(1) != 1))
@@ -451,6 +459,7 @@ PyObject* append_impl(PyObject* const* args) {
         const at::Tensor& f = tensor_of(args[kInvFreq], "inv_freq");
         if (f.scalar_type() != at::kDouble || f.dim() != 1 || !f.is_contiguous() || f.numel() < 1 || 2 * f.numel() > k.size(2))
             value_error("inv_freq must be float64 [rotary_dim / 2], rotary_dim at most head_dim");
+        need_no_grad(f, "inv_freq");
         need_reach(device, f, "inv_freq");
         p.inv_freq = static_cast<const double*>(f.data_ptr());
         p.rotary_dim = static_cast<int>(2 * f.numel());
@@ -483,7 +492,7 @@ PyObject* append_impl(PyObject* const* args) {
     } else if (args[kQOut] != Py_None) {
         value_error("out is for q");
     }
-    p.amplitude = static_cast<float>(float_of(args[kAmplitude]));
+    p.amplitude = static_cast<float>(number_of(args[kAmplitude], "amplitude"));
     p.interleaved = truth_of(args[kInterleaved]) ? 1 : 0;
     p.status = status_of(args[kAppendStatus], device);
     p.stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
@@ -539,6 +548,7 @@ PyObject* paged_impl(PyObject* const* args) {
     }
     if (truth_of(args[kPagedReturnLse])) lse = at::empty({T, H}, q.options().dtype(at::kFloat).layout(at::kStrided).requires_grad(false));
     if (args[kPagedSlopes] != Py_None) {
+        need_no_grad(tensor_of(args[kPagedSlopes], "alibi_slopes"), "alibi_slopes");
         slopes = tensor_of(args[kPagedSlopes], "alibi_slopes").to(device, at::kFloat).contiguous();
         if (slopes.numel() < H) value_error("alibi_slopes must hold a slope for each head");
     }
@@ -554,7 +564,7 @@ PyObject* paged_impl(PyObject* const* args) {
     }
     // (unsaid: as many as there are rows, or one)
     p.max_seqlen_q = args[kMaxSeqlenQ] != Py_None ? int_of(args[kMaxSeqlenQ]) : p.cache.cu_seqlens_q ? narrow_int(std::max<int64_t>(T, 1)) : 1;
-    p.softmax_scale = static_cast<float>(args[kPagedScale] != Py_None ? float_of(args[kPagedScale]) : 1.0 / std::sqrt(static_cast<double>(std::max<int64_t>(d, 1))));
+    p.softmax_scale = static_cast<float>(args[kPagedScale] != Py_None ? number_of(args[kPagedScale], "softmax_scale") : 1.0 / std::sqrt(static_cast<double>(std::max<int64_t>(d, 1))));
     p.is_causal = truth_of(args[kPagedCausal]) ? 1 : 0;
     window_of(args[kPagedWindow], &p.window_left, &p.window_right);
     p.alibi_slopes = slopes.defined() ? static_cast<const float*>(slopes.data_ptr()) : nullptr;

@@ -1,0 +1,44 @@
+"""The calls around a paged cache and autograd: nothing is recorded, so nothing that a gradient hangs on is taken or passed by."""
+import pytest
+import torch
+
+import paged_util as pu
+
+pytestmark = pytest.mark.gpu
+
+
+def fa():
+    import flash_attn_b200
+    return flash_attn_b200
+
+
+def made():
+    """Each call with its arguments, by name."""
+    t = torch.float16
+    lens = torch.tensor([20, 30], dtype=torch.int32).cuda()
+    k_pages, v_pages, table = pu.make_cache([20, 30], 16, 2, 64, t, seed=1)
+    f, _ = fa().rotary_frequencies(64)
+    rand = lambda *s: torch.randn(*s, device="cuda").to(t)  # noqa: E731
+    cache = dict(k_pages=k_pages, v_pages=v_pages, page_table=table, seqlens_k=lens)
+    one = lambda: torch.ones((), dtype=torch.float64, device="cuda")  # noqa: E731
+    return {
+        "rotary": (fa().rotary_embedding, dict(x=rand(2, 4, 64), positions=torch.arange(2, device="cuda"), inv_freq=f, amplitude=one(), out=rand(2, 4, 64))),
+        "append": (fa().paged_kv_append, dict(k=rand(2, 2, 64), v=rand(2, 2, 64), **cache, q=rand(2, 4, 64), inv_freq=f, amplitude=one(), out=rand(2, 4, 64))),
+        "attention": (fa().paged_attn_forward, dict(q=rand(2, 4, 64), **cache, softmax_scale=one() / 8, alibi_slopes=torch.ones(4, device="cuda"), out=rand(2, 4, 64)))}
+
+
+FLOATS = [("rotary", n) for n in ("x", "inv_freq", "amplitude", "out")] + [("append", n) for n in ("k", "v", "k_pages", "v_pages", "q", "inv_freq", "amplitude", "out")] + [
+    ("attention", n) for n in ("q", "k_pages", "v_pages", "softmax_scale", "alibi_slopes", "out")]
+
+
+@pytest.mark.parametrize("name, argument", FLOATS)
+def test_a_tensor_that_requires_grad_is_refused(name, argument):
+    call, args = made()[name]
+    call(**args)
+    args[argument] = args[argument].clone().requires_grad_()
+    with pytest.raises(ValueError, match=f"{argument} requires grad"):
+        call(**args)
+    with torch.no_grad():
+        call(**args)
+    args[argument] = args[argument].detach()
+    call(**args)
