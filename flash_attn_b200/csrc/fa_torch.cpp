@@ -6,6 +6,7 @@
 #include <Python.h>
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <cuda_runtime_api.h>
@@ -290,8 +291,9 @@ PyObject* forward(PyObject*, PyObject* const* args, Py_ssize_t n) {
     PyErr_Format(PyExc_ValueError, "%s %s", name, what);
     throw python_error_set();
 }
-// The kernels are not recorded by autograd: a gradient that would be lost in silence is refused.
+// The kernels are not recorded by autograd: a gradient or a tangent that would be lost in silence is refused.
 void need_no_grad(const at::Tensor& t, const char* name) {
+    if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined()) value_error_of(name, "has a forward-mode tangent: unpack it first");
     if (t.requires_grad() && at::GradMode::is_enabled()) value_error_of(name, "requires grad: call this under torch.no_grad() or inside an autograd Function");
 }
 // float(x) of a number or a tensor of one

@@ -11,7 +11,8 @@ The j-th of n new tokens has position `seqlens_k[b] - n + j`.  Rows behind the l
 Lengths and tables live on the device and are read there, so a step can be captured into a CUDA graph and replayed on new ones.
 A step of a layer is `q = paged_kv_append(k, v, ..., q=q, inv_freq=f)`, then `paged_attn_forward(q, ...)`.
 
-Nothing here is recorded by autograd: a tensor that requires grad, whichever argument it is, is refused while grad mode is on.  The gradient of
+Nothing here is recorded by autograd: a tensor that requires grad, whichever argument it is, is refused while grad mode is on, and so is
+one with a forward-mode tangent.  The gradient of
 rotary_embedding is rotary_embedding(grad, ..., inverse=True).
 """
 import ctypes

@@ -42,3 +42,20 @@ def test_a_tensor_that_requires_grad_is_refused(name, argument):
         call(**args)
     args[argument] = args[argument].detach()
     call(**args)
+
+
+@pytest.mark.parametrize("name, argument", FLOATS)
+def test_a_tensor_with_a_tangent_is_refused(name, argument):
+    from torch.autograd import forward_ad
+    call, args = made()[name]
+    with forward_ad.dual_level():
+        plain = args[argument]
+        args[argument] = forward_ad.make_dual(plain, torch.ones_like(plain))
+        with pytest.raises(ValueError, match=f"{argument} has a forward-mode tangent"):
+            call(**args)
+        with torch.no_grad(), pytest.raises(ValueError, match="tangent"):  # (no_grad leaves forward mode on)
+            call(**args)
+        args[argument] = forward_ad.unpack_dual(args[argument]).primal
+        call(**args)
+    args[argument] = plain
+    call(**args)
