@@ -296,6 +296,10 @@ void need_no_grad(const at::Tensor& t, const char* name) {
     if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined()) value_error_of(name, "has a forward-mode tangent: unpack it first");
     if (t.requires_grad() && at::GradMode::is_enabled()) value_error_of(name, "requires grad: call this under torch.no_grad() or inside an autograd Function");
 }
+// A caller's tensor was written to: autograd's check of what it has saved is told, as torch's own calls do (under no_grad too).
+void written(const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 // float(x) of a number or a tensor of one
 double number_of(PyObject* x, const char* name) {
     if (THPVariable_Check(x)) need_no_grad(THPVariable_Unpack(x), name);
@@ -387,6 +391,7 @@ PyObject* rotary_impl(PyObject* const* args) {
         rc = rotary(&p);
         Py_END_ALLOW_THREADS
         if (rc != FA_OK) return PyLong_FromLong(rc);
+        written(out);
     }
     return args[7] != Py_None ? Py_NewRef(args[7]) : THPVariable_Wrap(std::move(out));
 }
@@ -504,6 +509,8 @@ PyObject* append_impl(PyObject* const* args) {
         rc = append(&p);
         Py_END_ALLOW_THREADS
         if (rc != FA_OK) return PyLong_FromLong(rc);
+        for (int i = 0; i < 2; ++i) written(THPVariable_Unpack(args[kAppendCache + i]));
+        if (out.defined()) written(out);
     }
     return !out.defined() ? Py_NewRef(Py_None) : args[kQOut] != Py_None ? Py_NewRef(args[kQOut]) : THPVariable_Wrap(std::move(out));
 }
@@ -589,6 +596,7 @@ PyObject* paged_impl(PyObject* const* args) {
         rc = fwd(&p);
         Py_END_ALLOW_THREADS
         if (rc != FA_OK) return PyLong_FromLong(rc);
+        written(out);
     }
     PyObject* first = args[kPagedOut] != Py_None ? Py_NewRef(args[kPagedOut]) : THPVariable_Wrap(std::move(out));
     PyObject* second = !lse.defined() ? Py_NewRef(Py_None) : THPVariable_Wrap(std::move(lse));

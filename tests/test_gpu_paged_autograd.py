@@ -59,3 +59,32 @@ def test_a_tensor_with_a_tangent_is_refused(name, argument):
         call(**args)
     args[argument] = plain
     call(**args)
+
+
+@pytest.mark.parametrize("name, outputs", [("rotary", ["out"]), ("append", ["k_pages", "v_pages", "out"]), ("attention", ["out"])])
+def test_autograd_learns_what_was_written_to(name, outputs):
+    """A tensor that a graph has saved and a call has overwritten since is named by backward, not used."""
+    call, args = made()[name]
+    before = {n: x._version for n, x in args.items()}
+    with torch.no_grad():
+        call(**args)
+    assert {n for n, x in args.items() if x._version != before[n]} == set(outputs)
+    for n in outputs:
+        w = torch.ones((), dtype=args[n].dtype, device="cuda", requires_grad=True)
+        loss = (w * args[n]).float().sum()
+        call(**args)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    with torch.inference_mode():  # (tensors of inference mode count nothing)
+        args = {n: x.clone() for n, x in args.items()}
+        call(**args)
+
+
+def test_a_rotation_in_place_is_seen():
+    x = torch.randn(1, 2, 8, 64, device="cuda")
+    f, _ = fa().rotary_frequencies(64)
+    w = torch.ones((), device="cuda", requires_grad=True)
+    loss = (w * x).sum()
+    fa().rotary_embedding(x, torch.arange(8, device="cuda"), f, out=x)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
