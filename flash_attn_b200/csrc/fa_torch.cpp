@@ -503,7 +503,7 @@ PyObject* append_impl(PyObject* const* args) {
     p.interleaved = truth_of(args[kInterleaved]) ? 1 : 0;
     p.status = status_of(args[kAppendStatus], device);
     p.stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
-    if (k.numel() != 0) {
+    if (k.numel() != 0 || (out.defined() && out.numel() != 0)) {  // (pages without heads are refused where there is a Q to turn)
         int rc;
         Py_BEGIN_ALLOW_THREADS
         rc = append(&p);
