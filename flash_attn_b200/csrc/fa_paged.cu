@@ -263,6 +263,8 @@ int fa_paged_fwd(const fa_paged_fwd_params* p) {
     if (major != 10) return FA_ERR_NOT_SM100;
     const PagedLaunch l = plan_launch(p, sms);
     if (l.grid > 0x7fffffffLL) return FA_ERR_TOO_LARGE;
+    // (the rows of a chunk come by a tensor map, whose dimensions each have a stride)
+    if (!l.columns && ((p->tokens > 1 && p->q_stride[0] == 0) || (p->heads > 1 && p->q_stride[1] == 0))) return FA_ERR_INVALID_ARG;
     if (l.bytes > 0 && (!p->workspace || p->workspace_bytes < l.bytes)) return FA_ERR_WORKSPACE;
     if (l.bytes > 0 && (reinterpret_cast<uintptr_t>(p->workspace) & 15u)) return FA_ERR_INVALID_ARG;
     const fa_paged_kv& c = p->cache;

@@ -525,7 +525,7 @@ enum PagedArg {
 PyObject* paged_impl(PyObject* const* args) {
     const paged_fn fwd = reinterpret_cast<paged_fn>(bits_of(args[kPagedFn]));
     const paged_workspace_fn workspace_bytes = reinterpret_cast<paged_workspace_fn>(bits_of(args[kPagedWorkspaceFn]));
-    const at::Tensor& q = tensor_of(args[kPagedQ], "q");
+    at::Tensor q = tensor_of(args[kPagedQ], "q");
     if (!q.is_cuda()) value_error("paged_attn_forward needs CUDA tensors");
     if (q.dim() != 3) value_error("q must be [tokens, heads, head_dim]");
     need_no_grad(q, "q");
@@ -533,6 +533,7 @@ PyObject* paged_impl(PyObject* const* args) {
     const c10::Device device = q.device();
     const c10::cuda::OptionalCUDAGuard guard(device);
     const int64_t T = q.size(0), H = q.size(1), d = q.size(2);
+    if ((T > 1 && q.stride(0) == 0) || (H > 1 && q.stride(1) == 0)) q = q.contiguous();  // (broadcast rows: the chunk kernel takes none)
     fa_paged_fwd_params p;
     std::memset(&p, 0, sizeof p);
     p.cache = cache_of(args + kPagedCache, q, device);

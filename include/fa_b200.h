@@ -402,7 +402,8 @@ typedef struct fa_paged_fwd_params {
     int o_dtype;              /* cache.dtype, or FA_DTYPE_FP32 */
     int heads;                /* a multiple of cache.heads, at most 128 times it */
     int64_t tokens;
-    int64_t q_stride[2];      /* elements from one token and head to the next; multiples of 8 */
+    int64_t q_stride[2];      /* elements from one token and head to the next; multiples of 8, 0 (a broadcast row) only where
+                                 max_seqlen_q * heads / cache.heads is 16 at most */
     int64_t o_stride[2];      /* multiples of 4 */
     int max_seqlen_q;         /* most new tokens of a sequence: says which kernel suits, results do not depend on it */
     float softmax_scale;      /* > 0 */
