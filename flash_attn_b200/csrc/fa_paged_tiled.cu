@@ -218,22 +218,19 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                 ++answered;
             };
             int tt = 0, parts_with_tiles = 0;
-            for (int nth = 0;; ++nth) {
+            bool first = true;
+            for (int nth = 0;;) {
                 if (fail == 0 && __any_sync(0xffffffffu, *abort_flag != 0)) fail = 1;  // (no more than what was taken)
-                if (nth > 0) {
+                if (!first) {
                     ask();
                     answer();
                 }
+                first = false;
                 const int at = nth % kSegs;
                 if (nth >= kSegs && !wait_part(bar_seg_free + 8 * at, (nth / kSegs - 1) & 1)) { fail = 3; break; }
                 PagedSeg g;
-                bool have;
-                for (;;) {
-                    have = index >= 0 && line.find(a.plan, a.div_group, index, lane, &g);
-                    if (have || index < 0) break;
-                    ask();  // a CTA behind the last part need not start; one before it may still be taken
-                    answer();
-                }
+                const bool have = index >= 0 && line.find(a.plan, a.div_group, index, lane, &g);
+                if (!have && index >= 0) continue;  // (a CTA behind the last part need not start; one before it may still be taken)
                 if (!have) g.n_rows = 0;
                 if (lane == 0) {
                     segs[at] = g;
@@ -241,6 +238,7 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                     mbar_arrive(bar_seg_full + 8 * at);
                 }
                 __syncwarp();
+                ++nth;
                 if (!have) break;
                 if (g.n_tiles == 0) continue;
                 const int* table = a.page_table + g.b * a.table_stride;
