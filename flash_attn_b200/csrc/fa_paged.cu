@@ -68,7 +68,14 @@ PagedLaunch plan_launch(const fa_paged_fwd_params* p, int sms) {
     const int group = p->heads / c.heads;
     const long long rows = static_cast<long long>(std::min<int64_t>(p->max_seqlen_q, p->tokens)) * group;
     const int tile_rows = kTile / group * group;
+    // Up to 16 rows, a block of the few-rows kernel, go there.  (32 heads on 8 of 128 columns, 16 rows: 24 sequences of 500 .. 8000 keys 67 us,
+    // with one query tile 90, two 81; 4 of 30000 .. 60000 keys 119, 262, 261.  Two of its blocks, 32 rows: 89, 90, 75; and 150, 257, 257.
+    // Four, 64 rows: 154, 91, 76; and 319, 262, 203.)
     l.columns = rows == 1 ? 1 : rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 ? 16 : 0;
+    // One query tile, two CTAs an SM, where a sequence's rows fill no second one; above that two tiles share each K/V tile.  (Many short
+    // sequences, one tile and two: 256 of 20 new tokens, 32 heads on 8 of 128 columns: 77 and 117 us; 64 of 128, 32 heads of 64: 46 and 66.
+    // 192 rows in the 24 sequences above: 125 and 90.  Few blocks or long caches would be the faster for the second's one CTA an SM and
+    // two K/V stages below that, too: the 24 sequences with 128 rows 93 and 77.)
     l.query_tiles = l.columns ? 0 : rows <= tile_rows ? 1 : 2;
     l.rows = l.columns ? l.columns : l.query_tiles * tile_rows;
     l.wide = c.head_dim <= 64 ? 64 : 128;

@@ -11,6 +11,7 @@
 //
 // [64 x 32 heads on 8, 8192 keys each, d 128]: 322 us with pages of 16 tokens, 6.7 TB/s; 100 .. 8192 keys: 82 us, 5.4 TB/s (set-up 5 us, the
 // last parts 8); one sequence of 1000 keys: 13 us.  The code is kept short on purpose: what runs once is fetched from HBM first.
+// Spills at 168 registers (bytes stored): 130 and 90 with one column of D = 128 and 64, 24 with four, 8 with eight, none with sixteen.
 //
 // What the pool holds beyond a sequence is not known, and 0 * NaN is NaN: keys that no row sees have P = 0 by their scores, and
 // their rows of a V tile are overwritten with zeros before its MMAs, on the first and last tile of a block.

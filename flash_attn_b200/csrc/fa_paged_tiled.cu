@@ -12,8 +12,10 @@
 // What the pool holds beyond a sequence is not known, and 0 * NaN is NaN: rows of a V tile that no row of the block sees are
 // overwritten with zeros before its MMAs (first and last tile only).
 //
-// 2048 tokens over 32768 keys, 32 heads on 8, d 128: 960 us, 1.1 PFLOP/s, a KV tile of two query tiles 1.8 to 2.1 us (a chain of latencies of two
-// softmax warps a scheduler); six prompts of 200 .. 2048 tokens: 43 us, where parts of one to eight tiles begin and end.
+// 2048 tokens over 32768 keys, 32 heads on 8, d 128: twenty calls in a row 933 us each, 1.14 PFLOP/s, a thousand (under the power cap) 1042,
+// 1.02; a KV tile of two query tiles 1.8 to 2.1 us (a chain of latencies of two softmax warps a scheduler).  Six prompts of 200 .. 2048
+// tokens: 43 us, where parts of one to eight tiles begin and end.  Spills (bytes stored): 88 with two query tiles at D = 128, up to 16 at
+// D = 64, 200 to 250 with one (128 registers at launch).
 #include <algorithm>
 #include <atomic>
 #include <cuda_bf16.h>

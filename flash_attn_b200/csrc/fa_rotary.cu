@@ -8,7 +8,9 @@
 // The angle of a far position is large (a million radians at 2^20), so position * inv_freq in 32 bits would be wrong by a tenth of
 // a radian.  A turn is taken as 2^64 instead: inv_freq / 2 pi, less its whole turns, is rounded to a 64-bit fraction f, and
 // position * f in wrapping integer arithmetic IS the angle modulo a turn, off by position * 2^-53 turns (what the double holds).
-// Its upper 32 bits, as a signed number of half turns, are what sincospi is given.
+// Its upper 32 bits, as a signed number of half turns, are what sincospi is given: as a float of 24 bits, off by 2^-25 of a half turn at
+// most (9.4e-8 of |a| + |b|: thousands of times less than the rounding of a 16-bit result; fp32 results are off by 4.5e-8 on the whole, where
+// sines of 64-bit angles leave 3.4e-8).
 #include <algorithm>
 #include <cmath>
 #include <cuda_bf16.h>

@@ -5,7 +5,7 @@ The cache is a pool `k_pages`, `v_pages` [num_pages, heads_k, page_size, head_di
 dimensions, so a pool that is [num_pages, page_size, heads_k, head_dim] in memory is given as `pool.transpose(1, 2)`).  Token t of
 sequence b lies in page `page_table[b, t // page_size]` (int32 [batch, pages]), slot `t % page_size`; `seqlens_k` (int32 [batch])
 counts the tokens of each sequence, the new ones of this step included.  The new tokens of all sequences are rows one behind the
-other, `cu_seqlens_q[b] .. cu_seqlens_q[b + 1]` (int32 [batch + 1]) those of sequence b; without it there is one row a sequence.
+other, `cu_seqlens_q[b] .. cu_seqlens_q[b + 1]` (int32 [batch + 1], ascending) those of sequence b; without it there is one row a sequence.
 The j-th of n new tokens has position `seqlens_k[b] - n + j`.  Rows behind the last sequence are left as they were.
 
 Lengths and tables live on the device and are read there, so a step can be captured into a CUDA graph and replayed on new ones.
@@ -55,7 +55,10 @@ def rotary_embedding(x, positions, inv_freq, amplitude=1.0, interleaved=False, i
     piece; positions int32 or int64 [seqlen], [batch, seqlen] or [tokens]; inv_freq float64 [rotary_dim / 2] (rotary_frequencies).
     Pair i is columns (i, i + rotary_dim / 2), `interleaved`: (2 i, 2 i + 1); columns from rotary_dim on are copied.  `inverse`
     turns back, which is also the gradient's way: it multiplies by the transposed map.  `out` may be x (in place) or memory that
-    does not overlap it.  Angles are exact for any position (64-bit fixed point modulo a turn), the rest is in 32 bits."""
+    does not overlap it.
+
+    position * inv_freq is taken modulo a turn in 64-bit fixed point, so that far positions lose nothing; the angle that is left is
+    rounded to 32 bits for sine and cosine (an error of 1e-7 of the pair's |a| + |b|), and the products are in 32 bits."""
     call = _lib.rotary or (_lib.load_call() and _lib.rotary)
     done = call(x, positions, inv_freq, amplitude, interleaved, inverse, out)
     if type(done) is int:
@@ -88,8 +91,10 @@ def paged_attn_forward(q, k_pages, v_pages, page_table, seqlens_k, cu_seqlens_q=
     chunk of new tokens sees the cache and itself), `window` = (left, right) with -1 = unbounded, `alibi_slopes` fp32 [heads].
     A row that sees no key gets o = 0, lse = -inf.  `max_seqlen_q`: the most new tokens that a sequence brings, known to the host
     (unsaid: it may be as many as there are); it says which kernel suits, the results are right whatever it is.
-    lse is fp32 [tokens, heads].  Slots past a sequence's length may hold anything, and so may pages that its rows' masks hide
-    whole; a value that is not finite at a place that one of 128 rows of a tile sees may reach the others.
+    lse is fp32 [tokens, heads].  Scores, sums and o are in 32 bits, but each probability is rounded to q's dtype for the product with
+    V, as in flash_attn_forward and whatever `out_dtype` is.  Slots past a sequence's length may hold anything, and so may pages that
+    its rows' masks hide whole; a value of V that is not finite may reach all of the up to 256 rows (a row is a token and a query head
+    of one K/V head) of a block of which one sees it.
 
     `workspace`: room for partial results (allocated where it is missing or too small); two calls that may run at once need one
     each.  `status`: an int32 word on the device, zeroed by the caller: 400 where a visible page is not in the pool (the rows that

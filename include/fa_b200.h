@@ -314,7 +314,9 @@ int fa_ring_comm_destroy(void* comm);
  * Whatever they hold, no memory outside the tensors is touched: a negative length counts as 0, row numbers are clipped
  * to the rows there are, and a page that is not in the pool (or beyond the table's width) is never followed: see status.
  * (Where cu_seqlens_q does not ascend, rows that several sequences claim get what one of them gives, or stay as they were.)
- * Slots at or past seqlens_k[b], and pages of which no row sees a key, may hold anything.
+ * Slots at or past seqlens_k[b], and pages of which no row sees a key, may hold anything.  A value of V that is not finite reaches
+ * the rows that see it, and may reach the others of their block, whose share of it is zero: up to 256 rows (a row is a new token and
+ * one of the query heads of a K/V head) of a sequence.
  */
 typedef struct fa_paged_kv {
     void* k;                  /* device, dtype: [num_pages, heads, page_size, head_dim], in any order of the first three */
@@ -349,8 +351,9 @@ int fa_rotary_frequencies(int rotary_dim, double base, int kind, double factor, 
  *   y[a] = amplitude (x[a] cos theta - x[b] sin theta),  y[b] = amplitude (x[b] cos theta + x[a] sin theta)
  * for the columns (a, b) = (i, i + rotary_dim / 2), interleaved: (2 i, 2 i + 1); columns from rotary_dim on are copied.
  * inverse: sin theta -> -sin theta, the transposed map, which takes the gradient of y to that of x.
- * Angles are taken modulo a turn in 64-bit fixed point (exact to 2^-53 of a turn a position), sines, cosines and products are in
- * 32 bits, the result is rounded once. */
+ * Angles are taken modulo a turn in 64-bit fixed point (exact to 2^-53 of a turn a position).  From there on 32 bits: the angle is
+ * rounded to 2^-25 of a half turn for sine and cosine (1e-7 of |x[a]| + |x[b]|), and so are these, times amplitude, and the products.
+ * The result is rounded once to dtype. */
 typedef struct fa_rotary_params {
     const void* x;            /* device, dtype: [batch, heads, rows, head_dim], in any order of the first three */
     void* y;                  /* device, dtype; x itself (with the same strides), or memory that does not overlap it */
@@ -393,7 +396,9 @@ typedef struct fa_paged_append_params {
 int fa_paged_append(const fa_paged_append_params* p);
 
 /* Attention of the new tokens over their sequences' pages: causal, local, ALiBi as in fa_fwd, with the positions above; query head
- * h reads K/V head h / (heads / cache.heads).  A row that sees no key gets O = 0, LSE = -inf. */
+ * h reads K/V head h / (heads / cache.heads).  A row that sees no key gets O = 0, LSE = -inf.
+ * Scores, their maxima and sums and O are in 32 bits; each probability is rounded to cache.dtype for the product with V, as in fa_fwd
+ * and whatever o_dtype is (of sum p |v|, half a step of cache.dtype at most). */
 typedef struct fa_paged_fwd_params {
     fa_paged_kv cache;
     const void* q;            /* device, cache.dtype: [tokens, heads, head_dim] */
