@@ -98,7 +98,8 @@ def paged_attn_forward(q, k_pages, v_pages, page_table, seqlens_k, cu_seqlens_q=
 
     `workspace`: room for partial results (allocated where it is missing or too small); two calls that may run at once need one
     each.  `status`: an int32 word on the device, zeroed by the caller: 400 where a visible page is not in the pool (the rows that
-    met it are NaN), 300 + n where a bounded wait inside the kernel gave up (the results are undefined)."""
+    met it are NaN), 300 + n where a bounded wait inside the kernel gave up (the results are undefined; zero a workspace of your own
+    before its next use)."""
     call = _lib.paged or (_lib.load_call() and _lib.paged)
     done = call(q, k_pages, v_pages, page_table, seqlens_k, cu_seqlens_q, max_seqlen_q, softmax_scale, causal, window, alibi_slopes, out,
                 out_dtype, return_lse, workspace, status)
